@@ -252,6 +252,76 @@ QB200_API qb200_status qb200_swiglu_sliced(const float* gate, const float* up, u
                                            void* stream);
 QB200_API qb200_status qb200_sum_arrays(const float* parts, uint32_t count, uint64_t n, float* y, void* stream);
 
+/* ---- paged KV cache: append with rotation, attention, attention behind a shared prefix ----
+ * The serving forms of the support ops above, for batches whose sequences have different lengths, for prompts as well
+ * as single tokens, and for heads that share keys and values (the reference's attention is one dense block of equal
+ * lengths, crates/ml/quanta-nn/src/kernel.rs:64-175, crates/ml/quanta-nn/src/attention.rs).
+ *
+ * qb200_paged_kv: two pools [n_pages, kv_heads, page_size, head_dim] of dtype BF16 or F16, 16-byte aligned; page_size
+ *   16, 32, 64, 128 or 256; head_dim 64 or 128; status_dev: an int32 in device memory, zero-initialised.
+ * qb200_paged_batch: sequence b's keys are rows 0 .. kv_lens[b] - 1 of its pages table[b * table_stride + i] (i <
+ *   table_width).  kv_lens counts the call's new tokens.  cu_q [batch + 1]: the new tokens of sequence b are rows
+ *   [cu_q[b], cu_q[b + 1]) of the call's arrays, and they are the sequence's last ones; NULL: one new token per sequence
+ *   (then tokens == batch).  Rows from cu_q[batch] on belong to nobody and are left as they are in every output.
+ *   All of it lives on the device and is read there: a captured call follows later contents.
+ * A length that does not fit the call (negative, more keys than the table holds, cu_q falling or past `tokens`) is cut
+ * to what fits, a page number outside the pool reads as zeros and is not written, and a position outside the table of
+ * angles takes its last row; each is recorded in status_dev, reported once by qb200_paged_check, and the results of
+ * the sequence concerned mean nothing.  Nothing outside the given buffers is read or written.
+ *
+ * qb200_paged_rope_append: row t of q [tokens, heads * head_dim], k and v [tokens, kv_heads * head_dim] (x_dtype F32,
+ *   BF16 or F16; rows *_stride elements apart, so the parts of a fused projection can be passed as they are).  The first
+ *   rot_dim (even) columns of every q and k head are rotated, rotate-half (crates/ml/quanta-nn/src/rope.rs:23-58), by row
+ *   positions[t] of cos / sin [n_pos, rot_dim / 2] f32 (NULL: the row's place in its sequence); f32 arithmetic, one
+ *   rounding.  q -> q_out [tokens, heads * head_dim] of the cache's type, k and v -> the sequence's pages.  q and
+ *   q_out NULL with heads = 0: keys and values alone.  A token whose place would be negative (more new tokens than
+ *   keys) is not written.  Two tokens of one call must not have the same place.
+ * qb200_paged_attention: token at place p of its sequence sees keys 0 .. p (causal), the first prefix_lens[b] keys
+ *   too where prefix_lens is given, or all kv_lens[b] keys (causal = 0).  Score = scale * (q . k); softcap > 0: softcap *
+ *   tanh(score / softcap); slopes [heads] given: minus slopes[h] * |distance|.  heads is a multiple of kv_heads, head h
+ *   reads K/V head h / (heads / kv_heads).  q [tokens, heads * head_dim] of the cache's type (rows q_stride elements
+ *   apart, a multiple of 8; 16-byte aligned), out [tokens, heads * head_dim] dense; lse [tokens, heads] f32 or NULL: log of the sum of
+ *   exp(score).  A row that sees no key gives zeros and -inf.  f32 softmax and accumulation; the softmax weights enter the second
+ *   product in the cache's type.  scratch: qb200_paged_attention_scratch_floats floats, 16-byte aligned, not shared with
+ *   a call that may overlap.  A key or value of a sequence that is not finite reaches every row that is computed in
+ *   a tile with it, masked there or not; rows behind a sequence's last key may hold anything.
+ * qb200_shared_prefix_attention: every token of the batch sees the first prefix_len keys of prefix_pages (page numbers
+ *   of the same pools), then its own sequence's keys as above (causal, places counted from prefix_len on).  The prefix
+ *   is read once for all tokens.
+ * qb200_paged_check: waits for the stream, returns a recorded error once and clears it. */
+typedef struct qb200_paged_kv {
+    void* k_pages;
+    void* v_pages;
+    int32_t* status_dev;
+    uint64_t n_pages;
+    uint32_t page_size, kv_heads, head_dim;
+    int32_t dtype;
+} qb200_paged_kv;
+typedef struct qb200_paged_batch {
+    const int32_t* table;
+    const int32_t* kv_lens;
+    const int32_t* cu_q;
+    uint64_t table_stride;
+    uint32_t table_width, batch;
+} qb200_paged_batch;
+QB200_API qb200_status qb200_paged_rope_append(const qb200_paged_kv* kv, const qb200_paged_batch* batch, const void* q, const void* k,
+                                               const void* v, int32_t x_dtype, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
+                                               uint64_t tokens, uint32_t heads, const float* cos, const float* sin, uint32_t rot_dim,
+                                               uint64_t n_pos, const int32_t* positions, void* q_out, void* stream);
+QB200_API uint64_t qb200_paged_attention_scratch_floats(const qb200_paged_kv* kv, const qb200_paged_batch* batch, uint64_t tokens,
+                                                        uint32_t heads);
+QB200_API qb200_status qb200_paged_attention(const qb200_paged_kv* kv, const qb200_paged_batch* batch, const void* q, uint64_t q_stride,
+                                             uint64_t tokens, uint32_t heads, float scale, float softcap, const float* slopes,
+                                             const int32_t* prefix_lens, int32_t causal, float* scratch, void* out, float* lse,
+                                             void* stream);
+QB200_API uint64_t qb200_shared_prefix_scratch_floats(const qb200_paged_kv* kv, const qb200_paged_batch* batch, uint64_t prefix_len,
+                                                      uint64_t tokens, uint32_t heads);
+QB200_API qb200_status qb200_shared_prefix_attention(const qb200_paged_kv* kv, const qb200_paged_batch* batch,
+                                                     const int32_t* prefix_pages, uint64_t prefix_len, const void* q, uint64_t q_stride,
+                                                     uint64_t tokens, uint32_t heads, float scale, float softcap, const float* slopes,
+                                                     float* scratch, void* out, float* lse, void* stream);
+QB200_API qb200_status qb200_paged_check(const qb200_paged_kv* kv, void* stream);
+
 /* ---- fused all-gather for column-sharded layers (no counterpart in the reference: it has no
  * multi-GPU code, crates/ml/quanta-nn/PARITY.md:76-79) ----
  * Every rank of a node owns one gather buffer of the same layout (for example [world][layer][m][n]);

@@ -32,6 +32,15 @@ class StItem(ctypes.Structure):
     ]
 
 
+class PagedKv(ctypes.Structure):
+    _fields_ = [("k_pages", vp), ("v_pages", vp), ("status_dev", vp), ("n_pages", u64), ("page_size", u32), ("kv_heads", u32),
+                ("head_dim", u32), ("dtype", i32)]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [("table", vp), ("kv_lens", vp), ("cu_q", vp), ("table_stride", u64), ("table_width", u32), ("batch", u32)]
+
+
 # name -> (restype, argtypes); mirrors include/qb200.h one to one
 SIGNATURES = {
     "qb200_version": (cp, []),
@@ -58,6 +67,12 @@ SIGNATURES = {
     "qb200_sdpa_decode": (i32, [vp, vp, vp, u32, u32, u32, u32, u32, ctypes.c_float, vp, vp, vp]),
     "qb200_swiglu_sliced": (i32, [vp, vp, u64, u64, P(u32), u32, u32, vp, vp]),
     "qb200_sum_arrays": (i32, [vp, u32, u64, vp, vp]),
+    "qb200_paged_rope_append": (i32, [vp, vp, vp, vp, vp, i32, u64, u64, u64, u64, u32, vp, vp, u32, u64, vp, vp, vp]),
+    "qb200_paged_attention_scratch_floats": (u64, [vp, vp, u64, u32]),
+    "qb200_paged_attention": (i32, [vp, vp, vp, u64, u64, u32, ctypes.c_float, ctypes.c_float, vp, vp, i32, vp, vp, vp, vp]),
+    "qb200_shared_prefix_scratch_floats": (u64, [vp, vp, u64, u64, u32]),
+    "qb200_shared_prefix_attention": (i32, [vp, vp, vp, u64, vp, u64, u64, u32, ctypes.c_float, ctypes.c_float, vp, vp, vp, vp, vp]),
+    "qb200_paged_check": (i32, [vp, vp]),
     "qb200_peer_alloc": (i32, [u64, P(vp), ctypes.c_char_p]),
     "qb200_peer_open": (i32, [ctypes.c_char_p, P(vp)]),
     "qb200_peer_close": (i32, [vp]),

@@ -1,0 +1,172 @@
+// Shared pieces of the paged KV cache's kernels: which rows and keys a sequence has, the join of partial softmax
+// results, and the small PTX wrappers both attention kernels use.
+//
+// A cache is two pools [n_pages, kv_heads, page_size, hd]: the rows of one page and head are contiguous, so a tile
+// of keys is a few whole runs of page_size * hd elements.  Rows of a call are packed: row r of sequence b and K/V
+// head g is new token r / group, query head g * group + r % group, so that all the query heads that share a K/V head
+// read it together.
+//
+// The softmax runs in base 2 (scores times log2 e); m is the running maximum in those units, l the sum of
+// 2^(s - m), acc the sum of 2^(s - m) v, all in 32 bits.  A row that sees no key has m = -inf and l = 0.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "common.hpp"
+
+namespace qb {
+
+constexpr float PG_LOG2E = 1.4426950408889634f, PG_LN2 = 0.6931471805599453f;
+
+struct PgArgs {
+    const void* q;              // [tokens, q_stride], head h at column h * hd
+    const uint16_t* k;          // pools
+    const uint16_t* v;
+    const int32_t* table;       // [batch, table_stride] page numbers; the prefix phase: [width]
+    const int32_t* kv_lens;     // [batch]
+    const int32_t* cu_q;        // [batch + 1], or null: one token per sequence
+    const int32_t* prefix_lens; // [batch], or null
+    const float* slopes;        // [heads], or null
+    int32_t* status;
+    uint64_t q_stride, table_stride;
+    uint32_t n_pages, ps_log, width;  // page size = 1 << ps_log; width: pages a table row can hold
+    uint32_t batch, tokens, group, kv_heads;
+    uint32_t causal;
+    uint32_t shared;            // keys of a shared prefix: all tokens of the batch are one sequence that sees keys [0, shared)
+    float score_mul;            // log2 e * scale without a cap; scale / cap with one
+    float cap_mul;              // cap * log2 e, 0: no cap
+    // results: rows of `out` [tokens, heads * hd] joined with `base` where given, or rows of `rows_out`
+    uint16_t* out;
+    uint64_t out_stride;
+    float* lse;                 // [tokens, heads] or null
+    const float* base_acc;      // [tokens, heads, hd] and [tokens, heads, 2] (m, l): what a first phase left
+    const float* base_ml;
+    float* rows_acc;            // the same two, written instead of out by the first phase
+    float* rows_ml;
+    float* parts;               // partial results of units that several CTAs share
+    int32_t* meta;
+};
+
+struct PgSeq {
+    uint32_t q0, q_len, kv, see;  // rows [q0, q0 + q_len) of the batch; keys [0, kv); some row sees keys [0, see)
+    uint32_t prefix;
+};
+
+__device__ __forceinline__ void pg_report(int32_t* status, int32_t code) { atomicCAS(status, 0, code); }
+
+// What sequence b of the call has; lengths that do not fit the call are cut and reported.
+__device__ __forceinline__ PgSeq pg_seq(const PgArgs& a, uint32_t b) {
+    PgSeq s;
+    if (a.shared) {
+        int32_t n = a.cu_q ? a.cu_q[a.batch] : (int32_t)a.tokens;
+        s.q0 = 0;
+        s.q_len = n < 0 ? 0u : min((uint32_t)n, a.tokens);
+        s.kv = s.see = a.shared;
+        s.prefix = a.shared;
+        return s;
+    }
+    int32_t lo = (int32_t)b, hi = lo + 1, kv = a.kv_lens[b];
+    if (a.cu_q) {
+        lo = a.cu_q[b];
+        hi = a.cu_q[b + 1];
+    }
+    const int64_t room = (int64_t)a.width << a.ps_log;
+    if (lo < 0 || hi < lo || hi > (int32_t)a.tokens || kv < 0 || kv > room) {
+        pg_report(a.status, QB200_ERR_LENGTH);
+        lo = max(0, min(lo, (int32_t)a.tokens));
+        hi = max(lo, min(hi, (int32_t)a.tokens));
+        kv = kv < 0 ? 0 : (int32_t)(kv > room ? room : kv);
+    }
+    s.q0 = (uint32_t)lo;
+    s.q_len = (uint32_t)(hi - lo);
+    s.kv = s.see = (uint32_t)kv;
+    const int32_t p = a.prefix_lens ? a.prefix_lens[b] : 0;
+    s.prefix = a.causal ? (uint32_t)max(p, 0) : 0xFFFFFFFFu;
+    return s;
+}
+
+// Keys that token i of the sequence sees: its position is kv - q_len + i (negative for a sequence with fewer keys
+// than new tokens, whose first tokens see nothing).
+__device__ __forceinline__ uint32_t pg_limit(const PgSeq& s, uint32_t i) {
+    const int32_t to = (int32_t)s.kv - (int32_t)s.q_len + (int32_t)i + 1;
+    return min(s.kv, max((uint32_t)max(to, 0), s.prefix));
+}
+
+// Position of token i, counted from the first key that this phase reads (the bias by distance counts from it).
+__device__ __forceinline__ int32_t pg_position(const PgArgs& a, const PgSeq& s, uint32_t i) {
+    if (!a.shared) return (int32_t)s.kv - (int32_t)s.q_len + (int32_t)i;
+    // the prefix phase: row i is token i of the whole batch; its sequence's own keys follow the prefix
+    uint32_t b = i;
+    int32_t lo = (int32_t)i, hi = lo + 1;
+    if (a.cu_q) {
+        uint32_t l = 0, r = a.batch;  // the last b with cu_q[b] <= i
+        while (r - l > 1) {
+            const uint32_t mid = (l + r) >> 1;
+            if (a.cu_q[mid] <= (int32_t)i) l = mid; else r = mid;
+        }
+        b = l;
+        lo = a.cu_q[b];
+        hi = a.cu_q[b + 1];
+    }
+    const int64_t room = (int64_t)0x7FFFFFFF - a.shared;
+    return (int32_t)a.shared + (int32_t)min((int64_t)max(a.kv_lens[b], 0), room) - (hi - lo) + ((int32_t)i - lo);
+}
+
+// 2^x, flushing far below the range to zero.
+__device__ __forceinline__ float pg_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pg_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// cap * log2 e * tanh(x): 1 - 2 / (e^(2x) + 1) keeps an absolute error of a few 2^-24 of the cap over the whole range
+// (e^(2x) = 0 and inf give -1 and 1), which is what a score needs; tanh.approx errs by 2^-11 of it.
+__device__ __forceinline__ float pg_cap(float x, float cap_mul) {
+    const float e = pg_exp2(x * (2.0f * PG_LOG2E));
+    return fmaf(-2.0f * cap_mul, pg_rcp(e + 1.0f), cap_mul);
+}
+
+template <typename T> struct PgType;
+template <> struct PgType<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+};
+template <> struct PgType<__half> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ float widen(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+};
+
+// Attention over packed rows (paged_rows.cu): grid of CTAs and floats of partial results it may use.
+uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms);
+uint64_t pg_rows_part_floats(uint32_t grid, uint32_t hd);
+qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t grid, cudaStream_t st);
+
+template <typename... KArgs, typename... Args>
+static cudaError_t pg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, uint32_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+}  // namespace qb
