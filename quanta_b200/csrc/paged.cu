@@ -232,14 +232,46 @@ static qb200_status pg_sms(uint32_t* n) {
     return QB200_OK;
 }
 
-// Scratch of one phase: partial results, 16-byte rounded.
-static uint64_t pg_phase_floats(const PgArgs& a, uint32_t hd, uint32_t sms) { return pg_rows_part_floats(pg_rows_grid(a, sms), hd); }
+// Which kernels a phase needs: sequences of at most PG_FEW_ROWS packed rows go to one, all others to the other; where
+// only the device knows the lengths, both are launched.
+struct PgPlan {
+    bool few, many;
+    uint32_t min_rows, grid, splits;
+    uint64_t floats;  // scratch: the kernels follow one another and share it
+};
+static PgPlan pg_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
+    PgPlan p = {};
+    const uint64_t most = a.shared || a.cu_q ? (uint64_t)a.tokens * a.group : a.group;
+    p.many = most > PG_FEW_ROWS;
+    p.few = !p.many || (!a.shared && a.cu_q && a.group <= PG_FEW_ROWS);
+    p.min_rows = p.few ? PG_FEW_ROWS + 1 : 1;
+    if (p.few) {
+        p.grid = pg_rows_grid(a, sms);
+        p.floats = pg_rows_part_floats(p.grid, hd);
+    }
+    if (p.many) {
+        p.splits = pg_prompt_splits(a, sms);
+        const uint64_t n = pg_prompt_part_floats(a, p.splits, hd);
+        if (n > p.floats) p.floats = n;
+    }
+    p.floats = (p.floats + 3) / 4 * 4;
+    if (!p.floats) p.floats = 4;
+    return p;
+}
 
 static qb200_status pg_phase(PgArgs a, int dtype, uint32_t hd, uint32_t sms, float* scratch, cudaStream_t st) {
-    const uint32_t grid = pg_rows_grid(a, sms);
-    a.meta = reinterpret_cast<int32_t*>(scratch);
-    a.parts = scratch + (uint64_t)grid * 8;
-    return pg_rows_launch(a, dtype, hd, grid, st);
+    const PgPlan p = pg_plan(a, hd, sms);
+    if (p.many) {
+        a.parts = scratch;
+        const qb200_status r = pg_prompt_launch(a, dtype, hd, p.splits, p.min_rows, st);
+        if (r) return r;
+    }
+    if (p.few) {
+        a.meta = reinterpret_cast<int32_t*>(scratch);
+        a.parts = scratch + (uint64_t)p.grid * 8;
+        return pg_rows_launch(a, dtype, hd, p.grid, st);
+    }
+    return QB200_OK;
 }
 
 static void pg_scores(PgArgs& a, float scale, float softcap, const float* slopes) {
@@ -330,7 +362,7 @@ qb200_status qb200_paged_rope_append(const qb200_paged_kv* kv, const qb200_paged
 uint64_t qb200_paged_attention_scratch_floats(const qb200_paged_kv* kv, const qb200_paged_batch* batch, uint64_t tokens, uint32_t heads) {
     uint32_t sms = 0;
     if (!kv || !batch || kv->kv_heads == 0 || pg_sms(&sms)) return 0;
-    return pg_phase_floats(pg_args(kv, batch, tokens, heads), kv->head_dim, sms);
+    return pg_plan(pg_args(kv, batch, tokens, heads), kv->head_dim, sms).floats;
 }
 
 qb200_status qb200_paged_attention(const qb200_paged_kv* kv, const qb200_paged_batch* batch, const void* q, uint64_t q_stride, uint64_t tokens,
@@ -347,7 +379,6 @@ qb200_status qb200_paged_attention(const qb200_paged_kv* kv, const qb200_paged_b
     a.prefix_lens = prefix_lens;
     a.causal = causal ? 1 : 0;
     a.out = static_cast<uint16_t*>(out);
-    a.out_stride = (uint64_t)heads * kv->head_dim;
     a.lse = lse;
     pg_scores(a, scale, softcap, slopes);
     return pg_phase(a, kv->dtype, kv->head_dim, sms, scratch, static_cast<cudaStream_t>(stream));
@@ -371,8 +402,8 @@ uint64_t qb200_shared_prefix_scratch_floats(const qb200_paged_kv* kv, const qb20
     uint32_t sms = 0;
     if (!kv || !batch || kv->kv_heads == 0 || pg_sms(&sms)) return 0;
     const PgArgs own = pg_args(kv, batch, tokens, heads);
-    const uint64_t x = pg_phase_floats(own, kv->head_dim, sms);
-    const uint64_t y = pg_phase_floats(prefix_args(own, nullptr, prefix_len, kv->head_dim, nullptr), kv->head_dim, sms);
+    const uint64_t x = pg_plan(own, kv->head_dim, sms).floats;
+    const uint64_t y = pg_plan(prefix_args(own, nullptr, prefix_len, kv->head_dim, nullptr), kv->head_dim, sms).floats;
     return prefix_rows_floats(own, kv->head_dim) + (x > y ? x : y);  // the phases follow one another: one area for both
 }
 
@@ -399,7 +430,6 @@ qb200_status qb200_shared_prefix_attention(const qb200_paged_kv* kv, const qb200
     a.base_acc = p.rows_acc;
     a.base_ml = p.rows_ml;
     a.out = static_cast<uint16_t*>(out);
-    a.out_stride = (uint64_t)heads * kv->head_dim;
     a.lse = lse;
     return pg_phase(a, kv->dtype, kv->head_dim, sms, phase, s);
 }

@@ -17,6 +17,9 @@
 
 namespace qb {
 
+// Sequences of at most this many packed rows go to the kernel for few rows, the others to the prompt kernel.
+constexpr uint32_t PG_FEW_ROWS = 16;
+
 constexpr float PG_LOG2E = 1.4426950408889634f, PG_LN2 = 0.6931471805599453f;
 
 struct PgArgs {
@@ -38,7 +41,6 @@ struct PgArgs {
     float cap_mul;              // cap * log2 e, 0: no cap
     // results: rows of `out` [tokens, heads * hd] joined with `base` where given, or rows of `rows_out`
     uint16_t* out;
-    uint64_t out_stride;
     float* lse;                 // [tokens, heads] or null
     const float* base_acc;      // [tokens, heads, hd] and [tokens, heads, 2] (m, l): what a first phase left
     const float* base_ml;
@@ -149,10 +151,74 @@ template <> struct PgType<__half> {
     static __device__ __forceinline__ float widen(uint16_t b) { return __half2float(__ushort_as_half(b)); }
 };
 
+// Weight of a state with maximum m against the joint maximum M (a state without keys has none).
+__device__ __forceinline__ float pg_weight(float m, float M) { return m == -INFINITY ? 0.0f : pg_exp2(m - M); }
+
+// The end of one row's state (m, l): joined with what an earlier phase left and normalised, or kept for a later phase.
+// acc goes through pg_store4, four columns at a time.
+struct PgEnd {
+    float f, g;    // factors of this state's and the earlier phase's acc; 1 / l is in both
+    uint64_t row;
+};
+__device__ __forceinline__ PgEnd pg_end(const PgArgs& a, uint32_t token, uint32_t head, float m, float l, bool first) {
+    PgEnd e;
+    e.row = (uint64_t)token * a.group * a.kv_heads + head;
+    e.f = 1.0f;
+    e.g = 0.0f;
+    if (a.rows_acc) {
+        if (first) *reinterpret_cast<float2*>(a.rows_ml + e.row * 2) = make_float2(m, l);
+        return e;
+    }
+    if (a.base_acc) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.base_ml + e.row * 2);
+        const float M = fmaxf(m, ml.x);
+        e.f = pg_weight(m, M);
+        e.g = pg_weight(ml.x, M);
+        l = fmaf(l, e.f, ml.y * e.g);
+        m = M;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    e.f *= inv;
+    e.g *= inv;
+    if (a.lse && first) a.lse[e.row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * PG_LN2;
+    return e;
+}
+template <typename T, uint32_t HD>
+__device__ __forceinline__ void pg_store4(const PgArgs& a, const PgEnd& e, uint32_t col, float4 v) {
+    if (a.rows_acc) {
+        *reinterpret_cast<float4*>(a.rows_acc + e.row * HD + col) = v;
+        return;
+    }
+    v.x *= e.f;
+    v.y *= e.f;
+    v.z *= e.f;
+    v.w *= e.f;
+    if (a.base_acc) {
+        const float4 w = *reinterpret_cast<const float4*>(a.base_acc + e.row * HD + col);
+        v.x = fmaf(w.x, e.g, v.x);
+        v.y = fmaf(w.y, e.g, v.y);
+        v.z = fmaf(w.z, e.g, v.z);
+        v.w = fmaf(w.w, e.g, v.w);
+    }
+    uint2 o;
+    o.x = PgType<T>::pack(v.x, v.y);
+    o.y = PgType<T>::pack(v.z, v.w);
+    *reinterpret_cast<uint2*>(a.out + e.row * HD + col) = o;
+}
+template <typename T, uint32_t HD>
+__device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_t head, uint32_t col, float m, float l, float4 v) {
+    pg_store4<T, HD>(a, pg_end(a, token, head, m, l, col == 0), col, v);
+}
+
 // Attention over packed rows (paged_rows.cu): grid of CTAs and floats of partial results it may use.
 uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms);
 uint64_t pg_rows_part_floats(uint32_t grid, uint32_t hd);
 qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t grid, cudaStream_t st);
+// Attention for many rows (paged_prompt.cu): over how many ranges a unit's keys are cut, the floats of partial results
+// that takes, and the launch; min_rows: sequences of fewer packed rows are not its own.
+uint32_t pg_prompt_splits(const PgArgs& a, uint32_t sms);
+uint64_t pg_prompt_part_floats(const PgArgs& a, uint32_t splits, uint32_t hd);
+qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t splits, uint32_t min_rows, cudaStream_t st);
 
 template <typename... KArgs, typename... Args>
 static cudaError_t pg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, uint32_t smem, cudaStream_t st, Args... args) {

@@ -1,0 +1,699 @@
+// Paged attention for many rows per K/V head (prompts, chunks of prompts, large groups, a prefix shared by the batch):
+// bounded by the tensor pipe and, as closely, by the exponentials (128 x 128 scores cost 1024 cycles of either at head
+// dim 128: 4096 multiply-adds and 16 exponentials a cycle and SM).
+//
+// A unit is 256 packed rows of a sequence and one K/V head, over one of `splits` ranges of its keys; one CTA each, the
+// longest first.  The rows are two tiles of 128 whose steps alternate on the tensor pipe, so that one tile's products
+// run under the other's softmax.  Per step of 128 keys and tile: S = Q K^T (tcgen05.mma, both operands in shared
+// memory, accumulator in TMEM), a warpgroup turns S into P (a thread owns a row, so the row's maximum and sum need no
+// exchange), P goes back to TMEM over S in the cache's type, and O += P V takes it from there.  The running maximum a
+// row's weights are taken against moves only when the true one has passed it by 2^8 (weights then stay below 2^8, far from
+// any type's limit), so that the accumulator is rescaled in a few steps of the first tiles and hardly ever after.
+//
+// A block of at most 128 rows uses both warpgroups too: the second takes the odd tiles of keys of the same rows, and
+// the two results are joined in shared memory.
+//
+// Roles: warps 0-3 and 4-7 softmax and epilogue of the two tiles, warp 8 brings K and V tiles by TMA (one box per page
+// and 64 columns, 128-byte swizzle), warp 9 issues the products.  All waits are bounded and report through the cache's
+// status word.
+#include <cuda.h>
+#include <string>
+
+#include "paged.cuh"
+
+namespace qb {
+
+// Registers: 384 threads are launched with 168 each (64512 in all); the softmax warpgroups, which hold a row of 128
+// scores a thread, take 216, the third one keeps 72.
+constexpr uint32_t PP_THREADS = 384, PP_MORE = 216, PP_LESS = 72;
+static_assert(2 * PP_MORE + PP_LESS == 3 * 168, "the shares add up to what the launch gets");
+constexpr uint32_t PP_KEYS = 128, PP_ROWS = 128, PP_BLOCK = 256;
+constexpr uint32_t PP_POLLS = 1u << 22;
+template <uint32_t HD> struct PpShape {
+    static constexpr uint32_t PANEL = 128 * 128;            // 128 rows of 64 elements
+    static constexpr uint32_t TILE = PANEL * (HD / 64);     // a Q, K or V tile
+    static constexpr uint32_t STAGES = HD == 128 ? 5 : 8;
+    static constexpr uint32_t SMEM = 1024 + 2 * TILE + STAGES * TILE + 256;
+    static_assert(STAGES * TILE >= 128 * HD * 4 + 1024, "the second warpgroup's result fits the ring");
+    static constexpr uint32_t S_COLS = 128, O_COL = 256;    // TMEM: S of tile t at 128 t (P over its first 64), O at 256 + 128 t
+};
+
+__device__ __forceinline__ uint32_t pp_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void pp_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(pp_smem(bar)), "r"(count));
+}
+__device__ __forceinline__ void pp_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pp_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void pp_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(pp_smem(bar)), "r"(bytes) : "memory");
+}
+// Bounded wait for a barrier's phase; gives up at once when another role has.
+__device__ __forceinline__ bool pp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* gave_up) {
+    for (uint32_t i = 0; i < PP_POLLS; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(pp_smem(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((i & 63u) == 63u && *gave_up) return false;
+    }
+    *gave_up = 1;
+    return false;
+}
+__device__ __forceinline__ uint32_t pp_elect() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+__device__ __forceinline__ void pp_load(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+        "r"(x), "r"(y), "r"(z), "r"(w), "r"(pp_smem(bar))
+        : "memory");
+}
+// Shared-memory matrix descriptors, 128-byte swizzle.  K-major (Q, K): 8-row groups 1024 bytes apart.  MN-major (V as
+// [keys][columns]): groups of 8 keys 1024 bytes apart, panels of 64 columns 16 KB apart.
+__device__ __forceinline__ uint64_t pp_desc(uint32_t saddr, uint32_t lead) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void pp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void pp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+                 "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void pp_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(pp_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void pp_tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void pp_tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void pp_ld_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pp_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pp_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pp_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+// (x0, x1) * (m, m) + (c, c)
+__device__ __forceinline__ void pp_fma2(float& x0, float& x1, uint64_t m2, uint64_t c2) {
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tfma.rn.f32x2 t, t, %2, %3;\n\tmov.b64 {%0, %1}, t;\n\t}" : "+f"(x0), "+f"(x1) : "l"(m2), "l"(c2));
+}
+__device__ __forceinline__ void pp_add2(float& x0, float& x1, float y0, float y1) {
+    asm("{\n\t.reg .b64 t, u;\n\tmov.b64 t, {%0, %1};\n\tmov.b64 u, {%2, %3};\n\tadd.rn.f32x2 t, t, u;\n\tmov.b64 {%0, %1}, t;\n\t}"
+        : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
+}
+__device__ __forceinline__ uint64_t pp_pack2(float x) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+    return r;
+}
+
+struct PpArgs {
+    PgArgs g;
+    uint32_t splits, min_rows;
+    float* parts_acc;  // [splits][tokens * heads][hd] and [splits][tokens * heads][2], splits > 1
+    float* parts_ml;
+};
+
+__device__ __forceinline__ uint32_t pp_blocks(const PpArgs& a, uint32_t b) {
+    const PgSeq s = pg_seq(a.g, b);
+    const uint32_t rows = s.q_len * a.g.group;
+    return rows < a.min_rows ? 0 : (rows + PP_BLOCK - 1) / PP_BLOCK;
+}
+
+template <typename T, uint32_t HD, bool SCORED>
+__global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                                                const __grid_constant__ PpArgs pa) {
+    using S = PpShape<HD>;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sQ = smem;                    // [2][HD / 64 panels][128 rows][128 B]
+    uint8_t* sR = sQ + 2 * S::TILE;        // ring of K and V tiles
+    uint64_t* full = reinterpret_cast<uint64_t*>(sR + S::STAGES * S::TILE);
+    uint64_t* empty = full + S::STAGES;
+    uint64_t* q_full = empty + S::STAGES;
+    uint64_t* s_full = q_full + 1;         // [2] the tile's S is in TMEM (and every earlier product is complete)
+    uint64_t* p_full = s_full + 2;         // [2] the tile's P is in TMEM
+    uint64_t* o_full = p_full + 2;         // [2] the tile's O is complete
+    uint64_t* drained = o_full + 2;        // after giving up: the products in flight are complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    volatile uint32_t* gave_up = tmem_slot + 1;
+    const PgArgs& a = pa.g;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- which unit: blocks of all sequences, each sequence's last (longest) block first ----
+    __shared__ uint32_t s_seq, s_before, s_sum[PP_THREADS / 32];
+    const uint32_t seqs = a.shared ? 1 : a.batch, want = blockIdx.x / (a.kv_heads * pa.splits);
+    if (tid == 0) s_seq = 0xFFFFFFFFu;
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < seqs; b0 += PP_THREADS) {
+        const uint32_t b = b0 + tid, n = b < seqs ? pp_blocks(pa, b) : 0;
+        uint32_t incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            if (lane >= (uint32_t)o) incl += t;
+        }
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        uint32_t excl = before + incl - n;
+        for (uint32_t i = 0; i < PP_THREADS / 32; i++) {
+            if (i < warp) excl += s_sum[i];
+            before += s_sum[i];
+        }
+        if (excl <= want && want < excl + n) {
+            s_seq = b;
+            s_before = excl + n;
+        }
+        __syncthreads();
+        if (s_seq != 0xFFFFFFFFu) break;
+    }
+    if (s_seq == 0xFFFFFFFFu) return;  // the grid is an upper bound (the same for all threads)
+    const uint32_t b = s_seq, block = s_before - 1 - want;
+    const uint32_t kvh = blockIdx.x / pa.splits % a.kv_heads, split = blockIdx.x % pa.splits;
+    const PgSeq sq = pg_seq(a, b);
+    const uint32_t all_rows = sq.q_len * a.group, row0 = block * PP_BLOCK, rows = min(PP_BLOCK, all_rows - row0);
+    const uint32_t see = pg_limit(sq, (row0 + rows - 1) / a.group);  // keys the block's last token sees (the most)
+    const uint32_t n_all = (see + PP_KEYS - 1) / PP_KEYS;
+    const uint32_t t0 = (uint32_t)((uint64_t)n_all * split / pa.splits), t1 = (uint32_t)((uint64_t)n_all * (split + 1) / pa.splits), n = t1 - t0;
+    const bool dual = rows <= PP_ROWS;
+
+    if (tid == 0) {
+        for (uint32_t i = 0; i < S::STAGES; i++) {
+            pp_init(&full[i], 1);
+            pp_init(&empty[i], 1);
+        }
+        pp_init(q_full, 8);
+        pp_init(drained, 1);
+        for (uint32_t i = 0; i < 2; i++) {
+            pp_init(&s_full[i], 1);
+            pp_init(&p_full[i], 4);
+            pp_init(&o_full[i], 1);
+        }
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pp_smem(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pp_before();
+    __syncthreads();
+    pp_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PP_MORE));
+        // ---- softmax and epilogue: warpgroup w owns tile w (or, where the block is one tile, its keys' odd tiles) ----
+        const uint32_t w = warp >> 2, r = (warp & 3) * 32 + lane, wt = tid & 127;
+        const uint32_t first = dual ? 0 : w * PP_ROWS;  // the tile's first row of the block
+        const uint32_t t_rows = min(PP_ROWS, rows - first);
+        // Q rows to shared memory (rows past the last one are zeros)
+        if (!dual || w == 0) {
+            constexpr uint32_t CH = HD / 8;
+            for (uint32_t i = wt; i < PP_ROWS * CH; i += 128) {
+                const uint32_t qr = i / CH, c = i % CH;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (qr < t_rows) {
+                    const uint32_t row = row0 + first + qr, token = row / a.group, head = kvh * a.group + row % a.group;
+                    v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + token) * a.q_stride + (uint64_t)head * HD + c * 8);
+                }
+                *reinterpret_cast<uint4*>(sQ + w * S::TILE + (c >> 3) * S::PANEL + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) pp_arrive(q_full);
+
+        const uint32_t my = min(r, t_rows - 1);  // a row past the last one runs along with it and is not stored
+        const uint32_t row = row0 + first + my, token = row / a.group, head = kvh * a.group + row % a.group;
+        const uint32_t lim = pg_limit(sq, token);
+        const uint32_t lim_warp = __shfl_sync(0xFFFFFFFFu, lim, 0);  // the warp's least: limits grow with the row
+        float slope = 0.0f;
+        int32_t pos = 0;
+        if (SCORED && a.slopes) {
+            slope = a.slopes[head] * PG_LOG2E;
+            pos = pg_position(a, sq, token);
+        }
+        const uint32_t t_lane = tmem + (((warp & 3) * 32) << 16);
+        const uint32_t t_s = t_lane + w * S::S_COLS, t_o = t_lane + S::O_COL + w * 128;
+        const float c = SCORED ? 1.0f : a.score_mul;
+        const uint64_t c2 = pp_pack2(c);
+        const float slack = 8.0f / c;  // 2^8 in units of the raw score (the plain form has a positive scale)
+        float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        bool ok = true;
+        uint32_t it = 0;
+        for (uint32_t t = t0 + (dual ? w : 0); t < t1; t += dual ? 2 : 1, it++) {
+            if (!(ok = pp_wait(&s_full[w], it & 1, gave_up))) break;
+            pp_after();
+            float s[128];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) pp_tmem_ld32(t_s + i * 32, s + i * 32);
+            pp_ld_done();
+            const uint32_t key0 = t * PP_KEYS;
+            if (SCORED) {
+                if (a.cap_mul != 0.0f) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i] * a.score_mul, a.cap_mul);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 128; i++) s[i] *= a.score_mul;
+                }
+                if (a.slopes) {
+                    const float d0 = (float)(pos - (int32_t)key0);
+#pragma unroll
+                    for (uint32_t i = 0; i < 128; i++) s[i] = fmaf(-slope, fabsf(d0 - (float)i), s[i]);
+                }
+            }
+            if (key0 + PP_KEYS > lim_warp) {
+                const uint32_t left = lim > key0 ? lim - key0 : 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 128; i++) s[i] = i < left ? s[i] : -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (uint32_t i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (__any_sync(0xFFFFFFFFu, mt > m + slack)) {
+                const float mn = fmaxf(m, mt);
+                const float f = m == -INFINITY ? 0.0f : pg_exp2((m - mn) * c);
+                m = mn;
+                l0 *= f;
+                l1 *= f;
+                if (it) {  // the products up to the last step are complete: this step's S was issued behind them
+#pragma unroll 1
+                    for (uint32_t i = 0; i < HD; i += 32) {
+                        float o[32];
+                        pp_tmem_ld32(t_o + i, o);
+                        pp_ld_done();
+#pragma unroll
+                        for (uint32_t k = 0; k < 32; k++) o[k] *= f;
+                        pp_tmem_st32(t_o + i, reinterpret_cast<const uint32_t*>(o));
+                    }
+                    pp_st_done();
+                }
+            }
+            const uint64_t mc2 = pp_pack2(m == -INFINITY ? 0.0f : -m * c);
+            uint32_t pk[32];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; h++) {
+#pragma unroll
+                for (uint32_t i = 0; i < 64; i += 2) {
+                    float x0 = s[h * 64 + i], x1 = s[h * 64 + i + 1];
+                    pp_fma2(x0, x1, c2, mc2);
+                    x0 = pg_exp2(x0);
+                    x1 = pg_exp2(x1);
+                    pp_add2(l0, l1, x0, x1);
+                    pk[i >> 1] = PgType<T>::pack(x0, x1);
+                }
+                pp_tmem_st32(t_s + h * 32, pk);
+            }
+            pp_st_done();
+            pp_before();
+            __syncwarp();
+            if (lane == 0) pp_arrive(&p_full[w]);
+        }
+        // ---- epilogue ----
+        if (ok && it) ok = pp_wait(&o_full[w], 0, gave_up);
+        if (ok && dual && w == 1 && n) ok = pp_wait(&o_full[0], 0, gave_up);  // it writes where the other's products read
+        pp_after();
+        float l = l0 + l1, ml = m * c;  // (-inf stays -inf: c is positive)
+        float* other = reinterpret_cast<float*>(sR);  // [HD][128] and then m, l [128] each
+        if (dual && w == 1) {
+            // its part of the rows, for the first warpgroup; every load of the ring has been read by a product by now
+            if (ok && it) {
+#pragma unroll 1
+                for (uint32_t i = 0; i < HD; i += 32) {
+                    float o[32];
+                    pp_tmem_ld32(t_o + i, o);
+                    pp_ld_done();
+#pragma unroll
+                    for (uint32_t k = 0; k < 32; k++) other[(i + k) * 128 + r] = o[k];
+                }
+            }
+            if (ok) {
+                other[HD * 128 + r] = ml;
+                other[HD * 128 + 128 + r] = l;
+            }
+        }
+        if (dual) asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ok && (!dual || w == 0)) {
+            float f = 1.0f, g = 0.0f;
+            const bool join = dual && n > 1;
+            if (join) {
+                const float m1 = other[HD * 128 + r], M = fmaxf(ml, m1);
+                f = pg_weight(ml, M);
+                g = pg_weight(m1, M);
+                l = fmaf(l, f, other[HD * 128 + 128 + r] * g);
+                ml = M;
+            }
+            const uint64_t grow = (uint64_t)(sq.q0 + token) * a.group * a.kv_heads + head, all = (uint64_t)a.tokens * a.group * a.kv_heads;
+            const bool store = r < t_rows;
+            PgEnd e = {};
+            float* part = nullptr;
+            if (store) {
+                if (pa.splits > 1) {
+                    part = pa.parts_acc + ((uint64_t)split * all + grow) * HD;
+                    *reinterpret_cast<float2*>(pa.parts_ml + ((uint64_t)split * all + grow) * 2) = make_float2(ml, l);
+                } else {
+                    e = pg_end(a, sq.q0 + token, head, ml, l, true);
+                }
+            }
+#pragma unroll 1
+            for (uint32_t i = 0; i < HD; i += 32) {
+                float o[32];
+                if (it) {
+                    pp_tmem_ld32(t_o + i, o);
+                    pp_ld_done();
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 32; k++) {
+                    if (!it) o[k] = 0.0f;
+                    if (join) o[k] = fmaf(o[k], f, other[(i + k) * 128 + r] * g);
+                }
+                if (store) {
+#pragma unroll
+                    for (uint32_t k = 0; k < 32; k += 4) {
+                        const float4 v = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        if (part) *reinterpret_cast<float4*>(part + i + k) = v;
+                        else pg_store4<T, HD>(a, e, i + k, v);
+                    }
+                }
+            }
+        }
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PP_LESS));
+      if (warp == 8) {
+        // ---- K and V tiles by TMA: K0, then V of a step with K of the next one; in the one-tile form K0, K1 and K of the
+        // next but one.  A tile is a box per page (or half a page and less) and 64 columns; pages past the last key that is seen are not read.
+        const int32_t* table = a.table + (a.shared ? 0 : (uint64_t)b * a.table_stride);
+        const uint32_t ps = 1u << a.ps_log, box = min(ps, PP_KEYS), per = PP_KEYS / box;
+        const uint32_t ahead = dual ? 2 : 1;
+        uint32_t st = 0, count = 0;
+        bool ok = true;
+        auto page_of = [&](uint32_t t) -> int32_t {  // lane i: the page of the tile's i-th box
+            const uint32_t key = t * PP_KEYS + lane * box;
+            if (lane >= per || key >= see) return -1;
+            const int32_t p = table[key >> a.ps_log];
+            if ((uint32_t)p >= a.n_pages) {
+                pg_report(a.status, QB200_ERR_INVALID_PARAM);
+                return (int32_t)a.n_pages;  // outside the pool: the copy fills zeros
+            }
+            return p;
+        };
+        auto load = [&](const CUtensorMap* map, uint32_t t, int32_t page) {
+            if (count >= S::STAGES && !pp_wait(&empty[st], (count / S::STAGES - 1) & 1, gave_up)) { ok = false; return; }
+            const uint32_t boxes = min(per, (see - t * PP_KEYS + box - 1) / box);
+            if (lane == 0) pp_expect(&full[st], boxes * box * HD * 2);
+            __syncwarp();
+            if (lane < boxes) {
+                const uint32_t key = t * PP_KEYS + lane * box, dst = pp_smem(sR) + st * S::TILE + lane * box * 128;
+#pragma unroll
+                for (uint32_t p = 0; p < HD / 64; p++)
+                    pp_load(dst + p * S::PANEL, map, (int32_t)(p * 64), (int32_t)(key & (ps - 1)), (int32_t)kvh, page, &full[st]);
+            }
+            count++;
+            if (++st == S::STAGES) st = 0;
+        };
+        int32_t pages[3];  // of tiles t, t + 1, t + 2
+#pragma unroll
+        for (uint32_t i = 0; i < 3; i++) pages[i] = i < n ? page_of(t0 + i) : -1;
+        if (n) load(&kmap, t0, pages[0]);
+        if (ok && ahead == 2 && n > 1) load(&kmap, t0 + 1, pages[1]);
+        for (uint32_t i = 0; i < n && ok; i++) {
+            load(&vmap, t0 + i, pages[0]);
+            if (ok && i + ahead < n) load(&kmap, t0 + i + ahead, dual ? pages[2] : pages[1]);
+            pages[0] = pages[1];
+            pages[1] = pages[2];
+            pages[2] = i + 3 < n ? page_of(t0 + i + 3) : -1;
+        }
+        if (!ok)  // given up: let the copies in flight land before the memory goes
+            for (uint32_t i = count > S::STAGES ? count - S::STAGES : 0; i < count; i++)
+                for (uint32_t k = 0; k < 4096; k++) {
+                    uint32_t done;
+                    asm volatile(
+                        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                        : "=r"(done) : "r"(pp_smem(&full[i % S::STAGES])), "r"((i / S::STAGES) & 1) : "memory");
+                    if (done) break;
+                }
+      } else if (warp == 9 && n) {
+        // ---- products (the whole warp runs the loop, one elected lane issues) ----
+        const uint32_t elected = pp_elect();
+        constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        constexpr uint32_t base = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);
+        constexpr uint32_t idesc_s = base | ((PP_KEYS >> 3) << 17), idesc_o = base | (1u << 16) | ((HD >> 3) << 17);
+        const uint32_t q_s = pp_smem(sQ), r_s = pp_smem(sR);
+        auto scores = [&](uint32_t tile, uint32_t q_tile, uint32_t slot) {
+            if (elected) {
+                const uint64_t da = pp_desc(q_s + q_tile * S::TILE, 16), db = pp_desc(r_s + slot * S::TILE, 16);
+#pragma unroll
+                for (uint32_t kk = 0; kk < HD / 16; kk++) {
+                    const uint32_t off = (kk >> 2) * (S::PANEL >> 4) + (kk & 3) * 2;
+                    pp_mma_ss(tmem + tile * S::S_COLS, da + off, db + off, idesc_s, kk ? 1u : 0u);
+                }
+                pp_commit(&s_full[tile]);
+            }
+        };
+        auto values = [&](uint32_t tile, uint32_t slot, bool more, bool last) {
+            if (elected) {
+                const uint64_t db = pp_desc(r_s + slot * S::TILE, S::PANEL);
+#pragma unroll
+                for (uint32_t kk = 0; kk < PP_KEYS / 16; kk++)
+                    pp_mma_ts(tmem + S::O_COL + tile * 128, tmem + tile * S::S_COLS + kk * 8, db + kk * (2048 >> 4), idesc_o, (more || kk) ? 1u : 0u);
+                if (last) pp_commit(&o_full[tile]);
+            }
+        };
+        uint32_t count = 0;  // tiles taken from the ring, in the order they were loaded
+        auto next = [&](uint32_t& slot) -> bool {
+            slot = count % S::STAGES;
+            const bool got = pp_wait(&full[slot], (count / S::STAGES) & 1, gave_up);
+            count++;
+            return got;
+        };
+        // the last tile's rows of V behind the last key that is seen: zeros (their weights are zero, but a page may hold
+        // anything there, and 0 * NaN is NaN)
+        auto clean = [&](uint32_t t, uint32_t slot) {
+            const uint32_t valid = see - t * PP_KEYS;
+            if (valid >= PP_KEYS) return;
+            for (uint32_t i = valid * 8 + lane; i < PP_KEYS * 8; i += 32)
+#pragma unroll
+                for (uint32_t p = 0; p < HD / 64; p++) *reinterpret_cast<uint4*>(sR + slot * S::TILE + p * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        bool ok = pp_wait(q_full, 0, gave_up);
+        uint32_t k_slot = 0, v_slot = 0;
+        if (!dual) {
+            ok = ok && next(k_slot);
+            pp_after();
+            if (ok) {
+                scores(0, 0, k_slot);
+                scores(1, 1, k_slot);
+                if (elected) pp_commit(&empty[k_slot]);
+            }
+            for (uint32_t i = 0; i < n && ok; i++) {
+                const bool last = i + 1 == n;
+                if (!(ok = next(v_slot))) break;
+                if (last) clean(t0 + i, v_slot);
+                if (!last && !(ok = next(k_slot))) break;
+                for (uint32_t tile = 0; tile < 2; tile++) {
+                    if (!(ok = pp_wait(&p_full[tile], i & 1, gave_up))) break;
+                    pp_after();
+                    values(tile, v_slot, i > 0, last);
+                    if (tile == 1 && elected) pp_commit(&empty[v_slot]);
+                    if (!last) scores(tile, tile, k_slot);
+                }
+                if (ok && !last && elected) pp_commit(&empty[k_slot]);
+            }
+        } else {
+            for (uint32_t i = 0; i < 2 && i < n && ok; i++) {
+                if (!(ok = next(k_slot))) break;
+                pp_after();
+                scores(i, 0, k_slot);
+                if (elected) pp_commit(&empty[k_slot]);
+            }
+            for (uint32_t i = 0; i < n && ok; i++) {
+                const uint32_t tile = i & 1;
+                if (!(ok = next(v_slot))) break;
+                if (i + 1 == n) clean(t0 + i, v_slot);
+                if (i + 2 < n && !(ok = next(k_slot))) break;
+                if (!(ok = pp_wait(&p_full[tile], (i >> 1) & 1, gave_up))) break;
+                pp_after();
+                values(tile, v_slot, i > 1, i + 2 >= n);
+                if (elected) pp_commit(&empty[v_slot]);
+                if (i + 2 < n) {
+                    scores(tile, 0, k_slot);
+                    if (elected) pp_commit(&empty[k_slot]);
+                }
+            }
+        }
+        if (!ok) {  // given up: the products in flight read shared memory and TMEM
+            if (elected) pp_commit(drained);
+            for (uint32_t k = 0; k < 4096; k++) {
+                uint32_t done;
+                asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                             : "=r"(done) : "r"(pp_smem(drained)), "r"(0) : "memory");
+                if (done) break;
+            }
+        }
+      }
+    }
+    pp_before();
+    __syncthreads();
+    if (tid == 0 && *gave_up) pg_report(a.status, QB200_ERR_TIMEOUT);
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// Joins the ranges of keys of every row of the prompt kernel's sequences.
+template <typename T, uint32_t HD>
+__global__ void __launch_bounds__(128) k_paged_prompt_join(const __grid_constant__ PpArgs pa) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const PgArgs& a = pa.g;
+    constexpr uint32_t PER = HD / 4;
+    const uint32_t heads = a.group * a.kv_heads;
+    const uint64_t all = (uint64_t)a.tokens * heads, row = (uint64_t)blockIdx.x * (128 / PER) + threadIdx.x / PER;
+    if (row >= all) return;
+    const uint32_t token = (uint32_t)(row / heads), head = (uint32_t)(row % heads), col = (threadIdx.x % PER) * 4;
+    if (a.cu_q) {  // is the row one of theirs?  the last b with cu_q[b] <= token
+        if ((int32_t)token >= a.cu_q[a.batch]) return;
+        if (!a.shared) {
+            uint32_t lo = 0, hi = a.batch;
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (a.cu_q[mid] <= (int32_t)token) lo = mid; else hi = mid;
+            }
+            const PgSeq s = pg_seq(a, lo);
+            if (token < s.q0 || token - s.q0 >= s.q_len || s.q_len * a.group < pa.min_rows) return;
+        }
+    }
+    float M = -INFINITY, L = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t i = 0; i < pa.splits; i++) {
+        const float2 ml = *reinterpret_cast<const float2*>(pa.parts_ml + (i * all + row) * 2);
+        const float4 e = *reinterpret_cast<const float4*>(pa.parts_acc + (i * all + row) * HD + col);
+        const float Mn = fmaxf(M, ml.x), f = pg_weight(M, Mn), g = pg_weight(ml.x, Mn);
+        L = fmaf(L, f, ml.y * g);
+        v.x = fmaf(v.x, f, e.x * g);
+        v.y = fmaf(v.y, f, e.y * g);
+        v.z = fmaf(v.z, f, e.z * g);
+        v.w = fmaf(v.w, f, e.w * g);
+        M = Mn;
+    }
+    pg_emit<T, HD>(a, token, head, col, M, L, v);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------
+
+// Blocks of 256 rows that the call can have, over all sequences.
+static uint64_t pp_most_blocks(const PgArgs& a) {
+    const uint64_t rows = (uint64_t)a.tokens * a.group;
+    if (a.shared) return div_ceil(rows, PP_BLOCK);
+    if (!a.cu_q) return (uint64_t)a.batch * div_ceil(a.group, PP_BLOCK);
+    return rows / PP_BLOCK + (a.batch < a.tokens ? a.batch : a.tokens);
+}
+
+uint32_t pg_prompt_splits(const PgArgs& a, uint32_t sms) {
+    // fewer units than SMs: every unit's keys are cut so that all SMs have work, into ranges of at least two tiles
+    const uint64_t units = pp_most_blocks(a) * a.kv_heads, keys = a.shared ? a.shared : (uint64_t)a.width << a.ps_log;
+    const uint64_t by_keys = div_ceil(keys, 2 * PP_KEYS), by_sms = units ? sms / units : 1, s = by_keys < by_sms ? by_keys : by_sms;
+    return s > 1 ? (uint32_t)s : 1;
+}
+
+uint64_t pg_prompt_part_floats(const PgArgs& a, uint32_t splits, uint32_t hd) {
+    return splits > 1 ? (uint64_t)splits * a.tokens * a.group * a.kv_heads * (hd + 2) : 0;
+}
+
+typedef CUresult (*PpEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static PpEncodeFn pp_encode_fn() {
+    static PpEncodeFn fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PpEncodeFn>(p);
+    }
+    return fn;
+}
+
+template <typename T, uint32_t HD, bool SCORED>
+static qb200_status launch_prompt(const PpArgs& pa, uint32_t grid, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
+    static bool attr_set[64] = {};
+    int dev = 0;
+    QB_CUDA_TRY(cudaGetDevice(&dev));
+    if (!attr_set[dev & 63]) {
+        QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_prompt<T, HD, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PpShape<HD>::SMEM));
+        attr_set[dev & 63] = true;
+    }
+    QB_CUDA_TRY(pg_launch(k_paged_prompt<T, HD, SCORED>, dim3(grid), dim3(PP_THREADS), PpShape<HD>::SMEM, st, kmap, vmap, pa));
+    if (pa.splits > 1) {
+        const uint64_t rows = (uint64_t)pa.g.tokens * pa.g.group * pa.g.kv_heads, per = 128 / (HD / 4);
+        QB_CUDA_TRY(pg_launch(k_paged_prompt_join<T, HD>, dim3((uint32_t)((rows + per - 1) / per)), dim3(128), 0, st, pa));
+    }
+    return QB200_OK;
+}
+
+qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t splits, uint32_t min_rows, cudaStream_t st) {
+    PpEncodeFn enc = pp_encode_fn();
+    if (!enc) return fail(QB200_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled is not available from this driver");
+    const uint32_t ps = 1u << a.ps_log;
+    CUtensorMap map[2];
+    for (int i = 0; i < 2; i++) {
+        const cuuint64_t dims[4] = {hd, ps, a.kv_heads, a.n_pages};
+        const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)ps * hd * 2, (cuuint64_t)a.kv_heads * ps * hd * 2};
+        const cuuint32_t box[4] = {64, ps < PP_KEYS ? ps : PP_KEYS, 1, 1}, estr[4] = {1, 1, 1, 1};
+        const CUresult cr = enc(&map[i], dtype == QB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                                const_cast<uint16_t*>(i ? a.v : a.k), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (cr != CUDA_SUCCESS) return fail(QB200_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled failed with code " + std::to_string((int)cr));
+    }
+    PpArgs pa = {};
+    pa.g = a;
+    pa.splits = splits;
+    pa.min_rows = min_rows;
+    pa.parts_acc = a.parts;
+    pa.parts_ml = a.parts + (uint64_t)splits * a.tokens * a.group * a.kv_heads * hd;
+    const uint64_t units = pp_most_blocks(a) * a.kv_heads * splits;
+    if (units > 0x7FFFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, "paged attention: 2^31 blocks of rows or more");
+    const uint32_t grid = (uint32_t)units;
+    // a score that is not a positive multiple of q . k takes the general form (the plain one keeps its maximum in q . k)
+    const bool scored = a.cap_mul != 0.0f || a.slopes || !(a.score_mul > 1e-30f);
+    if (dtype == QB200_BF16) {
+        if (hd == 128) return scored ? launch_prompt<__nv_bfloat16, 128, true>(pa, grid, map[0], map[1], st) : launch_prompt<__nv_bfloat16, 128, false>(pa, grid, map[0], map[1], st);
+        return scored ? launch_prompt<__nv_bfloat16, 64, true>(pa, grid, map[0], map[1], st) : launch_prompt<__nv_bfloat16, 64, false>(pa, grid, map[0], map[1], st);
+    }
+    if (hd == 128) return scored ? launch_prompt<__half, 128, true>(pa, grid, map[0], map[1], st) : launch_prompt<__half, 128, false>(pa, grid, map[0], map[1], st);
+    return scored ? launch_prompt<__half, 64, true>(pa, grid, map[0], map[1], st) : launch_prompt<__half, 64, false>(pa, grid, map[0], map[1], st);
+}
+
+}  // namespace qb

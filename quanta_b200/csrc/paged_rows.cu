@@ -1,6 +1,6 @@
 // Paged attention for few rows per K/V head (single tokens, drafts): bounded by the bytes of K and V.
 //
-// A unit is (sequence, tile of 16 packed rows, K/V head); it has ceil(keys / 64) tiles of 64 keys.  The tiles of all
+// A unit is (sequence of at most 16 packed rows, K/V head); it has ceil(keys / 64) tiles of 64 keys.  The tiles of all
 // units, end to end, are cut into equal runs, one per CTA, so that ragged batches and one long sequence keep every SM
 // equally busy; a unit cut by a run's end leaves partial results (m, l, acc) that a second kernel joins.  The lengths
 // are read on the device, so a captured call follows them.
@@ -17,7 +17,8 @@
 
 namespace qb {
 
-constexpr uint32_t PR_WARPS = 4, PR_KEYS = 16, PR_TILE = PR_WARPS * PR_KEYS, PR_ROWS = 16;
+constexpr uint32_t PR_WARPS = 4, PR_KEYS = 16, PR_TILE = PR_WARPS * PR_KEYS, PR_ROWS = PG_FEW_ROWS;
+static_assert(PR_ROWS == 16, "the rows of one tensor instruction");
 template <uint32_t HD> struct PrShape {
     static constexpr uint32_t ROW = HD * 2, STAGE = 2 * PR_KEYS * ROW;  // bytes of a row; of a stage (K, then V)
     static constexpr uint32_t STAGES = HD == 128 ? 3 : 6, WARP = STAGES * STAGE, SMEM = PR_WARPS * WARP;
@@ -48,44 +49,12 @@ __device__ __forceinline__ void pr_mma(float (&d)[4], const uint32_t (&a)[4], ui
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Weight of a state with maximum m against the joint maximum M (a state without keys has none).
-__device__ __forceinline__ float pg_weight(float m, float M) { return m == -INFINITY ? 0.0f : pg_exp2(m - M); }
-
-// One row's finished state, four columns per thread: joined with what an earlier phase left, normalised and rounded
-// once, or kept whole for a later phase.
-template <typename T, uint32_t HD>
-__device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_t head, uint32_t col, float m, float l, float4 v) {
-    const uint64_t row = (uint64_t)token * a.group * a.kv_heads + head;
-    if (a.rows_acc) {
-        *reinterpret_cast<float4*>(a.rows_acc + row * HD + col) = v;
-        if (col == 0) *reinterpret_cast<float2*>(a.rows_ml + row * 2) = make_float2(m, l);
-        return;
-    }
-    if (a.base_acc) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.base_ml + row * 2);
-        const float4 w = *reinterpret_cast<const float4*>(a.base_acc + row * HD + col);
-        const float M = fmaxf(m, ml.x), f = pg_weight(m, M), g = pg_weight(ml.x, M);
-        l = fmaf(l, f, ml.y * g);
-        v.x = fmaf(v.x, f, w.x * g);
-        v.y = fmaf(v.y, f, w.y * g);
-        v.z = fmaf(v.z, f, w.z * g);
-        v.w = fmaf(v.w, f, w.w * g);
-        m = M;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint2 o;
-    o.x = PgType<T>::pack(v.x * inv, v.y * inv);
-    o.y = PgType<T>::pack(v.z * inv, v.w * inv);
-    *reinterpret_cast<uint2*>(a.out + token * a.out_stride + (uint64_t)head * HD + col) = o;
-    if (a.lse && col == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * PG_LN2;
-}
-
-// Tiles of one unit, and units, of sequence b.
+// Tiles of one unit of a sequence (a unit without keys still has one: it writes zeros), and of all its units; none
+// where the sequence has more rows than a unit holds (the prompt kernel takes those) or none.
 __device__ __forceinline__ uint32_t pr_tiles(const PgSeq& s) { return max(1u, (s.see + PR_TILE - 1) / PR_TILE); }
-__device__ __forceinline__ uint32_t pr_row_tiles(const PgArgs& a, const PgSeq& s) { return (s.q_len * a.group + PR_ROWS - 1) / PR_ROWS; }
-__device__ __forceinline__ uint64_t pr_weight(const PgArgs& a, uint32_t b) {
-    const PgSeq s = pg_seq(a, b);
-    return (uint64_t)pr_row_tiles(a, s) * a.kv_heads * pr_tiles(s);
+__device__ __forceinline__ uint64_t pr_weight(const PgArgs& a, const PgSeq& s) {
+    const uint64_t rows = (uint64_t)s.q_len * a.group;
+    return rows == 0 || rows > PG_FEW_ROWS ? 0 : (uint64_t)a.kv_heads * pr_tiles(s);
 }
 
 // Where the CTA's run of tiles lies: [run0, run1) of the total, and the sequence that holds tile run0 (first: its
@@ -100,7 +69,7 @@ __device__ __forceinline__ PrRun pr_find_run(const PgArgs& a, uint32_t seqs) {
     __shared__ uint32_t s_seq;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t sum = 0, mine = 0;
-    for (uint32_t b = tid; b < seqs; b += PR_WARPS * 32) sum += mine = pr_weight(a, b);
+    for (uint32_t b = tid; b < seqs; b += PR_WARPS * 32) sum += mine = pr_weight(a, pg_seq(a, b));
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) s_warp[warp] = sum;
@@ -120,7 +89,7 @@ __device__ __forceinline__ PrRun pr_find_run(const PgArgs& a, uint32_t seqs) {
     uint64_t before = 0;
     for (uint32_t b0 = 0; b0 < seqs; b0 += PR_WARPS * 32) {
         const uint32_t b = b0 + tid;
-        const uint64_t w = b < seqs ? (seqs <= PR_WARPS * 32 ? mine : pr_weight(a, b)) : 0;
+        const uint64_t w = b < seqs ? (seqs <= PR_WARPS * 32 ? mine : pr_weight(a, pg_seq(a, b))) : 0;
         uint64_t incl = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -167,21 +136,18 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a)
     uint64_t seq_first = run.first, at = run.run0;
     uint32_t slot = 0;  // the CTA's first partial unit goes to its slot 0, the last one to slot 1
     while (at < run.run1) {
-        uint32_t tiles = pr_tiles(sq), row_tiles = pr_row_tiles(a, sq);
-        while (at >= seq_first + (uint64_t)row_tiles * a.kv_heads * tiles) {  // on to the next sequence that has rows
-            seq_first += (uint64_t)row_tiles * a.kv_heads * tiles;
+        while (at >= seq_first + pr_weight(a, sq)) {  // on to the next sequence that has rows here
+            seq_first += pr_weight(a, sq);
             if (++b >= seqs) return;
             sq = pg_seq(a, b);
-            tiles = pr_tiles(sq);
-            row_tiles = pr_row_tiles(a, sq);
         }
-        const uint64_t unit = (at - seq_first) / tiles, unit_first = seq_first + unit * tiles;
-        const uint32_t kvh = (uint32_t)(unit % a.kv_heads), rt = (uint32_t)(unit / a.kv_heads);
+        const uint32_t tiles = pr_tiles(sq), kvh = (uint32_t)((at - seq_first) / tiles);
+        const uint64_t unit_first = seq_first + (uint64_t)kvh * tiles;
         const uint32_t t0 = (uint32_t)(at - unit_first);
         const uint32_t t1 = (uint32_t)min((uint64_t)tiles, run.run1 - unit_first);
         at = unit_first + t1;
-        const uint32_t rows = min(PR_ROWS, sq.q_len * a.group - rt * PR_ROWS);
-        const uint32_t see = pg_limit(sq, (rt * PR_ROWS + rows - 1) / a.group);  // keys the tile's last token sees (the most)
+        const uint32_t rows = sq.q_len * a.group;
+        const uint32_t see = pg_limit(sq, sq.q_len - 1);  // keys the last token sees (the most)
         const uint32_t te = min(t1, (see + PR_TILE - 1) / PR_TILE);
         const int32_t* table = a.table + (a.shared ? 0 : (uint64_t)b * a.table_stride);
 
@@ -194,12 +160,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a)
             const uint16_t* qp[2] = {nullptr, nullptr};
 #pragma unroll
             for (uint32_t i = 0; i < 2; i++) {
-                const uint32_t r = quad + 8 * i, row = rt * PR_ROWS + r;
+                const uint32_t r = quad + 8 * i;
                 lim[i] = 0;
                 slope[i] = 0.0f;
                 pos[i] = 0;
                 if (r < rows) {
-                    const uint32_t token = row / a.group, head = kvh * a.group + row % a.group;
+                    const uint32_t token = r / a.group, head = kvh * a.group + r % a.group;
                     lim[i] = pg_limit(sq, token);
                     qp[i] = static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + token) * a.q_stride + (uint64_t)head * HD;
                     if (SCORED && a.slopes) {
@@ -363,9 +329,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a)
             if (tid == 0 && t0 == 0) {
                 meta[1] = (int32_t)slot;
                 meta[2] = (int32_t)(sq.q0);
-                meta[3] = (int32_t)(rt * PR_ROWS);
-                meta[4] = (int32_t)rows;
-                meta[5] = (int32_t)kvh;
+                meta[3] = (int32_t)rows;
+                meta[4] = (int32_t)kvh;
                 // the CTA whose run holds the unit's last tile x: the largest c with total * c / ctas <= x
                 meta[0] = (int32_t)(((unit_first + tiles) * run.ctas - 1) / run.total);
             }
@@ -390,8 +355,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a)
                 v.w = fmaf(e.w, g, v.w);
             }
             if (whole) {
-                const uint32_t row = rt * PR_ROWS + r;
-                pg_emit<T, HD>(a, sq.q0 + row / a.group, kvh * a.group + row % a.group, col, M, L, v);
+                pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
             } else {
                 if (col == 0) {
                     part[r] = M;
@@ -414,7 +378,7 @@ __global__ void __launch_bounds__(128) k_paged_rows_join(const PgArgs a) {
     using S = PrShape<HD>;
     const int32_t* meta = a.meta + blockIdx.x * 8;
     if (meta[0] < 0) return;
-    const uint32_t slot0 = (uint32_t)meta[1], q0 = (uint32_t)meta[2], row0 = (uint32_t)meta[3], rows = (uint32_t)meta[4], kvh = (uint32_t)meta[5];
+    const uint32_t slot0 = (uint32_t)meta[1], q0 = (uint32_t)meta[2], rows = (uint32_t)meta[3], kvh = (uint32_t)meta[4];
     const uint32_t last = (uint32_t)meta[0];
     constexpr uint32_t PER = HD / 4, STEP = 128 / PER;
     const uint32_t r = blockIdx.y * STEP + threadIdx.x / PER, col = (threadIdx.x % PER) * 4;
@@ -433,15 +397,14 @@ __global__ void __launch_bounds__(128) k_paged_rows_join(const PgArgs a) {
         v.w = fmaf(v.w, f, e.w * g);
         M = Mn;
     }
-    const uint32_t row = row0 + r;
-    pg_emit<T, HD>(a, q0 + row / a.group, kvh * a.group + row % a.group, col, M, L, v);
+    pg_emit<T, HD>(a, q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
 uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms) {
     // two CTAs per SM, fewer where the call cannot have as many tiles
-    const uint64_t units = a.shared ? div_ceil((uint64_t)a.tokens * a.group, PR_ROWS) : (uint64_t)a.tokens * a.group / PR_ROWS + a.batch;
+    const uint64_t units = a.shared ? 1 : a.batch;
     const uint64_t keys = a.shared ? a.shared : (uint64_t)a.width << a.ps_log;
     const uint64_t most = units * a.kv_heads * (keys ? div_ceil(keys, PR_TILE) : 1);
     return (uint32_t)(most < 2 * sms ? (most ? most : 1) : 2 * sms);
