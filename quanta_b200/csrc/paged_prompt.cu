@@ -238,15 +238,26 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         const uint32_t t_rows = min(PP_ROWS, rows - first);
         // Q rows to shared memory (rows past the last one are zeros)
         if (!dual || w == 0) {
-            constexpr uint32_t CH = HD / 8;
-            for (uint32_t i = wt; i < PP_ROWS * CH; i += 128) {
-                const uint32_t qr = i / CH, c = i % CH;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (qr < t_rows) {
-                    const uint32_t row = row0 + first + qr, token = row / a.group, head = kvh * a.group + row % a.group;
-                    v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + token) * a.q_stride + (uint64_t)head * HD + c * 8);
+            // (eight rows' loads in flight per thread: one at a time costs a memory latency each, 13 us per unit)
+            constexpr uint32_t CH = HD / 8, STEP = 128 / CH, U = 8;
+            const uint32_t c = wt % CH;
+#pragma unroll 1
+            for (uint32_t i0 = wt / CH; i0 < PP_ROWS; i0 += STEP * U) {
+                uint4 v[U];
+#pragma unroll
+                for (uint32_t u = 0; u < U; u++) {
+                    const uint32_t qr = i0 + u * STEP;
+                    v[u] = make_uint4(0, 0, 0, 0);
+                    if (qr < t_rows) {
+                        const uint32_t row = row0 + first + qr, token = row / a.group, head = kvh * a.group + row % a.group;
+                        v[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + token) * a.q_stride + (uint64_t)head * HD + c * 8);
+                    }
                 }
-                *reinterpret_cast<uint4*>(sQ + w * S::TILE + (c >> 3) * S::PANEL + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v;
+#pragma unroll
+                for (uint32_t u = 0; u < U; u++) {
+                    const uint32_t qr = i0 + u * STEP;
+                    *reinterpret_cast<uint4*>(sQ + w * S::TILE + (c >> 3) * S::PANEL + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[u];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
@@ -597,16 +608,37 @@ __global__ void __launch_bounds__(128) k_paged_prompt_join(const __grid_constant
     }
     float M = -INFINITY, L = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t i = 0; i < pa.splits; i++) {
-        const float2 ml = *reinterpret_cast<const float2*>(pa.parts_ml + (i * all + row) * 2);
-        const float4 e = *reinterpret_cast<const float4*>(pa.parts_acc + (i * all + row) * HD + col);
-        const float Mn = fmaxf(M, ml.x), f = pg_weight(M, Mn), g = pg_weight(ml.x, Mn);
-        L = fmaf(L, f, ml.y * g);
-        v.x = fmaf(v.x, f, e.x * g);
-        v.y = fmaf(v.y, f, e.y * g);
-        v.z = fmaf(v.z, f, e.z * g);
-        v.w = fmaf(v.w, f, e.w * g);
+    constexpr uint32_t U = 6;  // ranges in flight
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < pa.splits; i0 += U) {
+        float2 ml[U];
+        float4 e[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const uint64_t i = min(i0 + u, pa.splits - 1);
+            ml[u] = *reinterpret_cast<const float2*>(pa.parts_ml + (i * all + row) * 2);
+            e[u] = *reinterpret_cast<const float4*>(pa.parts_acc + (i * all + row) * HD + col);
+        }
+        float Mn = M;
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) Mn = fmaxf(Mn, ml[u].x);
+        const float f = pg_weight(M, Mn);
         M = Mn;
+        L *= f;
+        v.x *= f;
+        v.y *= f;
+        v.z *= f;
+        v.w *= f;
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const float g = i0 + u < pa.splits ? pg_weight(ml[u].x, M) : 0.0f;
+            if (g == 0.0f) continue;  // no key there (or a weight below the smallest number)
+            L = fmaf(ml[u].y, g, L);
+            v.x = fmaf(e[u].x, g, v.x);
+            v.y = fmaf(e[u].y, g, v.y);
+            v.z = fmaf(e[u].z, g, v.z);
+            v.w = fmaf(e[u].w, g, v.w);
+        }
     }
     pg_emit<T, HD>(a, token, head, col, M, L, v);
 }

@@ -369,35 +369,70 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a)
     }
 }
 
-// Joins the partial results of the unit that starts in CTA blockIdx.x's run and ends in a later one's; a block takes
-// four of its rows.
+// Joins the partial results of the unit that starts in CTA blockIdx.x's run and ends in a later one's.  A block takes
+// the rows blockIdx.y, blockIdx.y + gridDim.y, ...; LANES groups of threads take every LANES-th part of a row (one
+// sequence's keys may be cut into dozens: taken one after the other, 37 parts cost 18 us) and meet in shared memory.
 template <typename T, uint32_t HD>
-__global__ void __launch_bounds__(128) k_paged_rows_join(const PgArgs a) {
+__global__ void __launch_bounds__(256) k_paged_rows_join(const PgArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     using S = PrShape<HD>;
-    const int32_t* meta = a.meta + blockIdx.x * 8;
-    if (meta[0] < 0) return;
-    const uint32_t slot0 = (uint32_t)meta[1], q0 = (uint32_t)meta[2], rows = (uint32_t)meta[3], kvh = (uint32_t)meta[4];
-    const uint32_t last = (uint32_t)meta[0];
-    constexpr uint32_t PER = HD / 4, STEP = 128 / PER;
-    const uint32_t r = blockIdx.y * STEP + threadIdx.x / PER, col = (threadIdx.x % PER) * 4;
-    if (r >= rows) return;
-    float M = -INFINITY, L = 0.0f;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t c = blockIdx.x; c <= last; c++) {
-        const float* p = a.parts + ((uint64_t)c * 2 + (c == blockIdx.x ? slot0 : 0)) * S::PART;
-        const float m = p[r], l = p[PR_ROWS + r];
-        const float4 e = *reinterpret_cast<const float4*>(p + 2 * PR_ROWS + r * HD + col);
-        const float Mn = fmaxf(M, m), f = pg_weight(M, Mn), g = pg_weight(m, Mn);
-        L = fmaf(L, f, l * g);
-        v.x = fmaf(v.x, f, e.x * g);
-        v.y = fmaf(v.y, f, e.y * g);
-        v.z = fmaf(v.z, f, e.z * g);
-        v.w = fmaf(v.w, f, e.w * g);
-        M = Mn;
+    constexpr uint32_t PER = HD / 4, LANES = 256 / PER, U = 3;
+    __shared__ float4 s_acc[LANES][PER];
+    __shared__ float s_m[LANES], s_l[LANES];
+    const int4 m0 = *reinterpret_cast<const int4*>(a.meta + blockIdx.x * 8);
+    if (m0.x < 0) return;
+    const uint32_t kvh = (uint32_t)a.meta[blockIdx.x * 8 + 4];
+    const uint32_t last = (uint32_t)m0.x, slot0 = (uint32_t)m0.y, q0 = (uint32_t)m0.z, rows = (uint32_t)m0.w;
+    const uint32_t lane = threadIdx.x / PER, col = (threadIdx.x % PER) * 4, lanes = min(LANES, last - blockIdx.x + 1);
+    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        float M = -INFINITY, L = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+        for (uint32_t c0 = blockIdx.x + lane; c0 <= last; c0 += LANES * U) {
+            float m[U], l[U];
+            float4 e[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {
+                const uint32_t c = min(c0 + u * LANES, last);
+                const float* p = a.parts + ((uint64_t)c * 2 + (c == blockIdx.x ? slot0 : 0)) * S::PART;
+                m[u] = c0 + u * LANES <= last ? p[r] : -INFINITY;
+                l[u] = p[PR_ROWS + r];
+                e[u] = *reinterpret_cast<const float4*>(p + 2 * PR_ROWS + r * HD + col);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {
+                if (c0 + u * LANES > last) continue;
+                const float Mn = fmaxf(M, m[u]), f = pg_weight(M, Mn), g = pg_weight(m[u], Mn);
+                L = fmaf(L, f, l[u] * g);
+                v.x = fmaf(v.x, f, e[u].x * g);
+                v.y = fmaf(v.y, f, e[u].y * g);
+                v.z = fmaf(v.z, f, e[u].z * g);
+                v.w = fmaf(v.w, f, e[u].w * g);
+                M = Mn;
+            }
+        }
+        s_acc[lane][threadIdx.x % PER] = v;
+        if (col == 0) {
+            s_m[lane] = M;
+            s_l[lane] = L;
+        }
+        __syncthreads();
+        if (lane == 0) {
+            for (uint32_t i = 1; i < lanes; i++) {
+                const float mi = s_m[i], Mn = fmaxf(M, mi), f = pg_weight(M, Mn), g = pg_weight(mi, Mn);
+                const float4 e = s_acc[i][threadIdx.x % PER];
+                L = fmaf(L, f, s_l[i] * g);
+                v.x = fmaf(v.x, f, e.x * g);
+                v.y = fmaf(v.y, f, e.y * g);
+                v.z = fmaf(v.z, f, e.z * g);
+                v.w = fmaf(v.w, f, e.w * g);
+                M = Mn;
+            }
+            pg_emit<T, HD>(a, q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
+        }
+        __syncthreads();
     }
-    pg_emit<T, HD>(a, q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
@@ -422,8 +457,8 @@ static qb200_status launch_rows(const PgArgs& a, uint32_t grid, cudaStream_t st)
         attr_set[dev & 63] = true;
     }
     QB_CUDA_TRY(pg_launch(k_paged_rows<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, a));
-    const uint32_t rows = (uint32_t)(a.tokens * (uint64_t)a.group < PR_ROWS ? a.tokens * a.group : PR_ROWS), step = 128 / (HD / 4);
-    QB_CUDA_TRY(pg_launch(k_paged_rows_join<T, HD>, dim3(grid, (rows + step - 1) / step), dim3(128), 0, st, a));
+    const uint64_t rows = a.cu_q || a.shared ? (uint64_t)a.tokens * a.group : a.group;
+    QB_CUDA_TRY(pg_launch(k_paged_rows_join<T, HD>, dim3(grid, (uint32_t)(rows < 8 ? rows : 8)), dim3(256), 0, st, a));
     return QB200_OK;
 }
 

@@ -21,6 +21,10 @@ import torch
 from . import _lib as L
 from .quant import QuantError, check as _check
 
+# The pieces of torch.cuda.device / current_stream that cost 0.1 us instead of 1.5 and 2 (a decode step makes dozens of calls).
+_device_now = getattr(torch._C, "_cuda_getDevice", None)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
 _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 
 
@@ -68,11 +72,12 @@ class PagedKVCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self.c = L.PagedKv(k.data_ptr(), v.data_ptr(), self.status.data_ptr(), n_pages, page_size, kv_heads, head_dim, _DTYPE[k.dtype])
         self._ref = ctypes.byref(self.c)
+        self._index = k.device.index if k.is_cuda else -1
+        self._scale = 1.0 / math.sqrt(head_dim)
 
     def check(self) -> None:
         """Waits for the current stream and raises what a kernel recorded (once)."""
-        with torch.cuda.device(self.device):
-            _check(L.load().qb200_paged_check(self._ref, torch.cuda.current_stream(self.device).cuda_stream))
+        _run(self, L.load().qb200_paged_check, self._ref)
 
 
 class PagedBatch:
@@ -90,18 +95,34 @@ class PagedBatch:
         for t in (table, kv_lens) if cu_q is None else (table, kv_lens, cu_q):
             _want(t.dtype == torch.int32 and t.device == cache.device and t.stride(-1) == 1, "PagedBatch: int32 tensors on the cache's device, rows contiguous")
         _want(b == 1 or table.stride(0) >= width, "PagedBatch: the table's rows overlap")
-        self.cache, self.table, self.kv_lens, self.cu_q = cache, table, kv_lens, cu_q
+        self.cache, self.table, self.kv_lens, self.cu_q, self.size = cache, table, kv_lens, cu_q, b
         self.c = L.PagedBatch(table.data_ptr(), kv_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), max(table.stride(0), width), width, b)
         self._ref = ctypes.byref(self.c)
+        self._floats = {}  # scratch sizes by shape of the call
 
 
-def _rows(x: torch.Tensor, width: int, device, what: str):
-    """x is [tokens, width] with contiguous columns on the cache's device; returns its row stride."""
-    if x.dim() != 2 or x.shape[1] != width or (x.stride(1) != 1 and width > 1):
-        _bad(f"{what} must be [tokens, {width}] with contiguous columns, got {list(x.shape)}", L.ERR_LENGTH)
-    if x.device != device:
-        _bad(f"{what} is on {x.device}, the cache on {device}")
-    return x.stride(0) if x.shape[0] > 1 else max(width, x.stride(0))
+def _run(cache: PagedKVCache, fn, *args) -> None:
+    """fn(*args, stream) with the cache's device current, on its current stream."""
+    index = cache._index
+    if index < 0:
+        _bad("the cache is not on a CUDA device", L.ERR_CUDA)
+    if _device_now is not None and _stream_of is not None and _device_now() == index:
+        status = fn(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if status:
+        _check(status)
+
+
+def _rows(x: torch.Tensor, heads: int, cache: PagedKVCache, what: str) -> Tuple[int, int, int]:
+    """(tokens, heads, row stride) of x ``[tokens, heads * head_dim]`` with contiguous columns; heads = 0: as many as there are."""
+    hd, shape = cache.head_dim, x.shape
+    if len(shape) != 2 or shape[1] != (heads * hd if heads else shape[1] // hd * hd) or shape[1] == 0 or x.stride(1) != 1:
+        _bad(f"{what} must be [tokens, {heads or 'heads'} * {hd}] with contiguous columns, got {list(shape)}", L.ERR_LENGTH)
+    if x.device != cache.device:
+        _bad(f"{what} is on {x.device}, the cache on {cache.device}")
+    return shape[0], shape[1] // hd, x.stride(0) if shape[0] > 1 else max(shape[1], x.stride(0))
 
 
 def _small(x: Optional[torch.Tensor], dtype, n: int, device, what: str) -> int:
@@ -119,15 +140,13 @@ def paged_rope_append(batch: PagedBatch, q: Optional[torch.Tensor], k: torch.Ten
     (all the same; rows may be strided, such as the parts of a fused projection); ``cos``, ``sin [n_pos, rot_dim / 2]``
     from ``rope_table``; ``positions [tokens]`` int32 (default: the token's place in its sequence).  q may be None."""
     cache = batch.cache
-    dev, hd = cache.device, cache.head_dim
-    tokens, kw = k.shape[0], cache.kv_heads * hd
-    ks, vs = _rows(k, kw, dev, "paged_rope_append: k"), _rows(v, kw, dev, "paged_rope_append: v")
-    heads = qs = 0
-    if q is not None:
-        heads = q.shape[-1] // hd
-        qs = _rows(q, heads * hd, dev, "paged_rope_append: q")
-    _want(v.shape[0] == tokens and (q is None or q.shape[0] == tokens), "paged_rope_append: q, k and v differ in tokens", L.ERR_LENGTH)
-    _want(k.dtype in _DTYPE and v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "paged_rope_append: q, k and v must be f32, bf16 or f16, all the same",
+    dev = cache.device
+    tokens, _, ks = _rows(k, cache.kv_heads, cache, "paged_rope_append: k")
+    v_tokens, _, vs = _rows(v, cache.kv_heads, cache, "paged_rope_append: v")
+    q_tokens, heads, qs = (tokens, 0, 0) if q is None else _rows(q, 0, cache, "paged_rope_append: q")
+    _want(v_tokens == tokens == q_tokens, "paged_rope_append: q, k and v differ in tokens", L.ERR_LENGTH)
+    x_dtype = _DTYPE.get(k.dtype)
+    _want(x_dtype is not None and v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "paged_rope_append: q, k and v must be f32, bf16 or f16, all the same",
           L.ERR_NOT_SUPPORTED)
     _want(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous() and
           cos.device == sin.device == dev, "paged_rope_append: cos and sin must be contiguous f32 [n_pos, rot_dim / 2] on the cache's device")
@@ -135,40 +154,45 @@ def paged_rope_append(batch: PagedBatch, q: Optional[torch.Tensor], k: torch.Ten
     if q is None:
         _want(q_out is None, "paged_rope_append: q_out without q")
     elif q_out is None:
-        q_out = torch.empty(tokens, heads * hd, dtype=cache.dtype, device=dev)
+        q_out = torch.empty(tokens, heads * cache.head_dim, dtype=cache.dtype, device=dev)
     else:
         _want(q_out.shape == q.shape and q_out.dtype == cache.dtype and q_out.device == dev and q_out.is_contiguous(),
               "paged_rope_append: q_out must be contiguous, of q's shape and the cache's type")
-    with torch.cuda.device(dev):
-        _check(L.load().qb200_paged_rope_append(cache._ref, batch._ref, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], qs, ks,
-                                                vs, tokens, heads, cos.data_ptr(), sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], pos,
-                                                0 if q is None else q_out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
+    _run(cache, L.load().qb200_paged_rope_append, cache._ref, batch._ref, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), x_dtype, qs, ks, vs,
+         tokens, heads, cos.data_ptr(), sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], pos, 0 if q is None else q_out.data_ptr())
     return q_out
 
 
 def _attend(who: str, batch: PagedBatch, q: torch.Tensor, slopes, out, lse):
     """The checks that both attentions share: (tokens, heads, q's row stride, pointer of slopes, out, pointer of lse)."""
     cache = batch.cache
-    dev, hd = cache.device, cache.head_dim
-    heads = q.shape[-1] // hd
-    qs = _rows(q, heads * hd, dev, who + ": q")
-    tokens = q.shape[0]
+    dev = cache.device
+    tokens, heads, qs = _rows(q, 0, cache, who)
     if q.dtype != cache.dtype:
         _bad(f"{who}: q is {q.dtype}, the cache {cache.dtype}", L.ERR_NOT_SUPPORTED)
     if out is None:
-        out = torch.empty(tokens, heads * hd, dtype=cache.dtype, device=dev)
+        out = torch.empty(q.shape, dtype=cache.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != cache.dtype or out.device != dev or not out.is_contiguous():
         _bad(f"{who}: out must be contiguous, of q's shape and the cache's type")
     if lse is not None and (lse.shape != (tokens, heads) or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous()):
         _bad(f"{who}: lse must be contiguous f32 [{tokens}, {heads}]")
-    return tokens, heads, qs, _small(slopes, torch.float32, heads, dev, who + ": slopes"), out, 0 if lse is None else lse.data_ptr()
+    return tokens, heads, qs, _small(slopes, torch.float32, heads, dev, who), out, 0 if lse is None else lse.data_ptr()
 
 
-def _scratch(who: str, scratch: Optional[torch.Tensor], floats: int, device) -> torch.Tensor:
+def _scratch(who: str, batch: PagedBatch, scratch: Optional[torch.Tensor], size_of, *shape) -> torch.Tensor:
+    """The call's workspace: the caller's, or one of its own from torch's allocator (which keeps calls on different
+    streams and in different captured graphs apart)."""
+    cache = batch.cache
+    floats = batch._floats.get(shape)
+    if floats is None:
+        if cache._index < 0:
+            _bad("the cache is not on a CUDA device", L.ERR_CUDA)
+        with torch.cuda.device(cache._index):
+            floats = batch._floats[shape] = size_of(cache._ref, batch._ref, *shape)
     if scratch is None:
-        return torch.empty(floats, dtype=torch.float32, device=device)
-    if scratch.dtype != torch.float32 or scratch.device != device or not scratch.is_contiguous() or scratch.numel() < floats:
-        _bad(f"{who}: scratch must be {floats} contiguous f32 values on {device}", L.ERR_LENGTH)
+        return torch.empty(floats, dtype=torch.float32, device=cache.device)
+    if scratch.dtype != torch.float32 or scratch.device != cache.device or not scratch.is_contiguous() or scratch.numel() < floats:
+        _bad(f"{who}: scratch must be {floats} contiguous f32 values on {cache.device}", L.ERR_LENGTH)
     return scratch
 
 
@@ -182,13 +206,11 @@ def paged_attention(batch: PagedBatch, q: torch.Tensor, scale: Optional[float] =
     f32 receives the log of each row's sum of exp(score).  A row that sees no key gives zeros and -inf."""
     cache = batch.cache
     tokens, heads, qs, sl, out, lp = _attend("paged_attention", batch, q, slopes, out, lse)
-    pl = _small(prefix_lens, torch.int32, batch.c.batch, cache.device, "paged_attention: prefix_lens")
+    pl = _small(prefix_lens, torch.int32, batch.size, cache.device, "paged_attention: prefix_lens")
     lib = L.load()
-    with torch.cuda.device(cache.device):
-        scratch = _scratch("paged_attention", scratch, lib.qb200_paged_attention_scratch_floats(cache._ref, batch._ref, tokens, heads), cache.device)
-        _check(lib.qb200_paged_attention(cache._ref, batch._ref, q.data_ptr(), qs, tokens, heads, 1.0 / math.sqrt(cache.head_dim) if scale is None else scale,
-                                         softcap, sl, pl, 1 if causal else 0, scratch.data_ptr(), out.data_ptr(), lp,
-                                         torch.cuda.current_stream(cache.device).cuda_stream))
+    scratch = _scratch("paged_attention", batch, scratch, lib.qb200_paged_attention_scratch_floats, tokens, heads)
+    _run(cache, lib.qb200_paged_attention, cache._ref, batch._ref, q.data_ptr(), qs, tokens, heads, cache._scale if scale is None else scale, softcap, sl, pl,
+         1 if causal else 0, scratch.data_ptr(), out.data_ptr(), lp)
     return out
 
 
@@ -205,10 +227,7 @@ def shared_prefix_attention(batch: PagedBatch, q: torch.Tensor, prefix_pages: to
     _want(prefix_pages.dim() == 1 and prefix_pages.dtype == torch.int32 and prefix_pages.is_contiguous() and prefix_pages.device == cache.device and
           prefix_pages.shape[0] >= need, f"shared_prefix_attention: {prefix_len} keys need {need} contiguous int32 page numbers on {cache.device}", L.ERR_LENGTH)
     lib = L.load()
-    with torch.cuda.device(cache.device):
-        scratch = _scratch("shared_prefix_attention", scratch, lib.qb200_shared_prefix_scratch_floats(cache._ref, batch._ref, prefix_len, tokens, heads),
-                           cache.device)
-        _check(lib.qb200_shared_prefix_attention(cache._ref, batch._ref, prefix_pages.data_ptr(), prefix_len, q.data_ptr(), qs, tokens, heads,
-                                                 1.0 / math.sqrt(cache.head_dim) if scale is None else scale, softcap, sl, scratch.data_ptr(),
-                                                 out.data_ptr(), lp, torch.cuda.current_stream(cache.device).cuda_stream))
+    scratch = _scratch("shared_prefix_attention", batch, scratch, lib.qb200_shared_prefix_scratch_floats, prefix_len, tokens, heads)
+    _run(cache, lib.qb200_shared_prefix_attention, cache._ref, batch._ref, prefix_pages.data_ptr(), prefix_len, q.data_ptr(), qs, tokens, heads,
+         cache._scale if scale is None else scale, softcap, sl, scratch.data_ptr(), out.data_ptr(), lp)
     return out
