@@ -65,6 +65,14 @@ __device__ __forceinline__ bool pp_wait(uint64_t* bar, uint32_t parity, volatile
     *gave_up = 1;
     return false;
 }
+// After giving up: a short wait for what is still in flight.
+__device__ __forceinline__ void pp_land(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < 4096; i++) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(pp_smem(bar)), "r"(parity) : "memory");
+        if (ok) return;
+    }
+}
 __device__ __forceinline__ uint32_t pp_elect() {
     uint32_t e;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
@@ -133,6 +141,30 @@ __device__ __forceinline__ uint64_t pp_pack2(float x) {
     return r;
 }
 
+__device__ __forceinline__ void pp_mul2(float& x0, float& x1, uint64_t m2) {
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tmul.rn.f32x2 t, t, %2;\n\tmov.b64 {%0, %1}, t;\n\t}" : "+f"(x0), "+f"(x1) : "l"(m2));
+}
+// tanh of a pair with |x| <= 1/2: x (1 + u P(u)), u = x^2, P the cubic that is best there (absolute error 4.3e-9, fitted
+// by reweighted least squares), on the multiply-add pipe: seven instructions a pair, where the exponential and the
+// reciprocal of the general form would triple the load of the pipe that already bounds the softmax.
+__device__ __forceinline__ void pp_tanh2(float& x0, float& x1, uint64_t c3, uint64_t c2, uint64_t c1, uint64_t c0, uint64_t one) {
+    asm("{\n\t.reg .b64 x, u, p;\n\t"
+        "mov.b64 x, {%0, %1};\n\t"
+        "mul.rn.f32x2 u, x, x;\n\t"
+        "fma.rn.f32x2 p, u, %2, %3;\n\t"
+        "fma.rn.f32x2 p, p, u, %4;\n\t"
+        "fma.rn.f32x2 p, p, u, %5;\n\t"
+        "fma.rn.f32x2 p, p, u, %6;\n\t"
+        "mul.rn.f32x2 x, x, p;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(x0), "+f"(x1) : "l"(c3), "l"(c2), "l"(c1), "l"(c0), "l"(one));
+}
+__device__ __forceinline__ uint64_t pp_pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
 struct PpArgs {
     PgArgs g;
     uint32_t splits, min_rows;
@@ -160,9 +192,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     uint64_t* empty = full + S::STAGES;
     uint64_t* q_full = empty + S::STAGES;
     uint64_t* s_full = q_full + 1;         // [2] the tile's S is in TMEM (and every earlier product is complete)
-    uint64_t* p_full = s_full + 2;         // [2] the tile's P is in TMEM
-    uint64_t* o_full = p_full + 2;         // [2] the tile's O is complete
-    uint64_t* drained = o_full + 2;        // after giving up: the products in flight are complete
+    uint64_t* p_full = s_full + 2;         // [2][2] half of the tile's P (64 keys) is in TMEM
+    uint64_t* o_full = p_full + 4;         // [2] the tile's O is complete
+    uint64_t* cleaned = o_full + 2;        // the last tile of V has zeros behind its last key
+    uint64_t* drained = cleaned + 1;       // after giving up: the products in flight are complete
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile uint32_t* gave_up = tmem_slot + 1;
     const PgArgs& a = pa.g;
@@ -212,10 +245,12 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             pp_init(&empty[i], 1);
         }
         pp_init(q_full, 8);
+        pp_init(cleaned, 1);
         pp_init(drained, 1);
         for (uint32_t i = 0; i < 2; i++) {
             pp_init(&s_full[i], 1);
-            pp_init(&p_full[i], 4);
+            pp_init(&p_full[2 * i], 4);
+            pp_init(&p_full[2 * i + 1], 4);
             pp_init(&o_full[i], 1);
         }
         *gave_up = 0;
@@ -228,7 +263,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     pp_before();
     __syncthreads();
     pp_after();
-    const uint32_t tmem = *tmem_slot;
+    // all 512 columns are this CTA's, so they start at 0; a constant keeps the products' addresses in uniform registers
+    constexpr uint32_t tmem = 0;
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PP_MORE));
@@ -276,9 +312,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         }
         const uint32_t t_lane = tmem + (((warp & 3) * 32) << 16);
         const uint32_t t_s = t_lane + w * S::S_COLS, t_o = t_lane + S::O_COL + w * 128;
-        const float c = SCORED ? 1.0f : a.score_mul;
+        // the factor that the exponential still has to apply: cap, or the whole scale of the plain form
+        const float c = !SCORED ? a.score_mul : a.slopes || a.cap_mul == 0.0f ? 1.0f : a.cap_mul;
         const uint64_t c2 = pp_pack2(c);
-        const float slack = 8.0f / c;  // 2^8 in units of the raw score (the plain form has a positive scale)
+        const float slack = 8.0f / c;  // 2^8 in units of the score (c is positive)
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         bool ok = true;
         uint32_t it = 0;
@@ -291,17 +328,50 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             pp_ld_done();
             const uint32_t key0 = t * PP_KEYS;
             if (SCORED) {
+                if (a.cap_mul != 0.0f || !a.slopes) {
+                    const uint64_t mul2 = pp_pack2(a.score_mul);
+#pragma unroll
+                    for (uint32_t i = 0; i < 128; i += 2) pp_mul2(s[i], s[i + 1], mul2);
+                }
                 if (a.cap_mul != 0.0f) {
+                    float far[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i] * a.score_mul, a.cap_mul);
-                } else {
+                    for (uint32_t i = 0; i < 128; i += 8)
 #pragma unroll
-                    for (uint32_t i = 0; i < 128; i++) s[i] *= a.score_mul;
+                        for (uint32_t k = 0; k < 4; k++) far[k] = fmaxf(fmaxf(far[k], fabsf(s[i + k])), fabsf(s[i + 4 + k]));
+                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) <= 0.5f))) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i], 1.0f);
+                    } else {
+                        const uint64_t k3 = pp_pack2(0.017005980014801025f), k2 = pp_pack2(-0.05292436107993126f), k1 = pp_pack2(0.13323938846588135f),
+                                       k0 = pp_pack2(-0.33333051204681396f), one = pp_pack2(1.0f);
+#pragma unroll
+                        for (uint32_t i = 0; i < 128; i += 2) pp_tanh2(s[i], s[i + 1], k3, k2, k1, k0, one);
+                    }
                 }
                 if (a.slopes) {
-                    const float d0 = (float)(pos - (int32_t)key0);
+                    const uint64_t up2 = pp_pack2(a.cap_mul != 0.0f ? a.cap_mul : a.score_mul);
+                    const int32_t d = pos - (int32_t)key0;
+                    if (__all_sync(0xFFFFFFFFu, d >= (int32_t)PP_KEYS - 1)) {  // no key behind the row's own place: linear in the key
+                        uint64_t off[4];
+                        const float df = (float)d;
 #pragma unroll
-                    for (uint32_t i = 0; i < 128; i++) s[i] = fmaf(-slope, fabsf(d0 - (float)i), s[i]);
+                        for (uint32_t k = 0; k < 4; k++) off[k] = pp_pair(slope * (float)(2 * k), slope * (float)(2 * k + 1));
+#pragma unroll
+                        for (uint32_t i = 0; i < 128; i += 8) {
+                            const float at = slope * ((float)i - df);
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; k++) {
+                                asm("{\n\t.reg .b64 t, x;\n\tmov.b64 t, {%2, %2};\n\tadd.rn.f32x2 t, t, %3;\n\tmov.b64 x, {%0, %1};\n\t"
+                                    "fma.rn.f32x2 x, x, %4, t;\n\tmov.b64 {%0, %1}, x;\n\t}"
+                                    : "+f"(s[i + 2 * k]), "+f"(s[i + 2 * k + 1]) : "f"(at), "l"(off[k]), "l"(up2));
+                            }
+                        }
+                    } else {
+                        const float up = a.cap_mul != 0.0f ? a.cap_mul : a.score_mul, d0 = (float)d;
+#pragma unroll
+                        for (uint32_t i = 0; i < 128; i++) s[i] = fmaf(-slope, fabsf(d0 - (float)i), s[i] * up);
+                    }
                 }
             }
             if (key0 + PP_KEYS > lim_warp) {
@@ -311,7 +381,11 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (uint32_t i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+            for (uint32_t i = 4; i < 124; i += 8)
+#pragma unroll
+                for (uint32_t k = 0; k < 4; k++) mx[k] = fmaxf(fmaxf(mx[k], s[i + k]), s[i + 4 + k]);  // one three-way maximum
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], s[124 + k]);
             const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             if (__any_sync(0xFFFFFFFFu, mt > m + slack)) {
                 const float mn = fmaxf(m, mt);
@@ -345,18 +419,20 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     pp_add2(l0, l1, x0, x1);
                     pk[i >> 1] = PgType<T>::pack(x0, x1);
                 }
+                // the product with V begins with the first half while the second one is computed
                 pp_tmem_st32(t_s + h * 32, pk);
+                pp_st_done();
+                pp_before();
+                __syncwarp();
+                if (lane == 0) pp_arrive(&p_full[2 * w + h]);
             }
-            pp_st_done();
-            pp_before();
-            __syncwarp();
-            if (lane == 0) pp_arrive(&p_full[w]);
         }
         // ---- epilogue ----
         if (ok && it) ok = pp_wait(&o_full[w], 0, gave_up);
         if (ok && dual && w == 1 && n) ok = pp_wait(&o_full[0], 0, gave_up);  // it writes where the other's products read
         pp_after();
-        float l = l0 + l1, ml = m * c;  // (-inf stays -inf: c is positive)
+        // (c is positive; a row that has seen no key may have collected weights of 2^-127)
+        float l = m == -INFINITY ? 0.0f : l0 + l1, ml = m * c;
         float* other = reinterpret_cast<float*>(sR);  // [HD][128] and then m, l [128] each
         if (dual && w == 1) {
             // its part of the rows, for the first warpgroup; every load of the ring has been read by a product by now
@@ -467,114 +543,110 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             pages[2] = i + 3 < n ? page_of(t0 + i + 3) : -1;
         }
         if (!ok)  // given up: let the copies in flight land before the memory goes
-            for (uint32_t i = count > S::STAGES ? count - S::STAGES : 0; i < count; i++)
-                for (uint32_t k = 0; k < 4096; k++) {
-                    uint32_t done;
-                    asm volatile(
-                        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                        : "=r"(done) : "r"(pp_smem(&full[i % S::STAGES])), "r"((i / S::STAGES) & 1) : "memory");
-                    if (done) break;
-                }
+            for (uint32_t i = count > S::STAGES ? count - S::STAGES : 0; i < count; i++) pp_land(&full[i % S::STAGES], (i / S::STAGES) & 1);
       } else if (warp == 9 && n) {
-        // ---- products (the whole warp runs the loop, one elected lane issues) ----
-        const uint32_t elected = pp_elect();
-        constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-        constexpr uint32_t base = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);
-        constexpr uint32_t idesc_s = base | ((PP_KEYS >> 3) << 17), idesc_o = base | (1u << 16) | ((HD >> 3) << 17);
-        const uint32_t q_s = pp_smem(sQ), r_s = pp_smem(sR);
-        auto scores = [&](uint32_t tile, uint32_t q_tile, uint32_t slot) {
-            if (elected) {
-                const uint64_t da = pp_desc(q_s + q_tile * S::TILE, 16), db = pp_desc(r_s + slot * S::TILE, 16);
+        // ---- products: one thread waits and issues (its branches are its own; the operands' addresses are constants but
+        // for the ring slot) ----
+        if (pp_elect()) {
+            constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr uint32_t base = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);
+            constexpr uint32_t idesc_s = base | ((PP_KEYS >> 3) << 17), idesc_o = base | (1u << 16) | ((HD >> 3) << 17);
+            const uint64_t q_desc = pp_desc(pp_smem(sQ), 16), k_desc = pp_desc(pp_smem(sR), 16), v_desc = pp_desc(pp_smem(sR), S::PANEL);
+            auto scores = [&](uint32_t tile, uint32_t q_tile, uint32_t slot) {
+                const uint64_t da = q_desc + q_tile * (S::TILE >> 4), db = k_desc + slot * (S::TILE >> 4);
 #pragma unroll
                 for (uint32_t kk = 0; kk < HD / 16; kk++) {
                     const uint32_t off = (kk >> 2) * (S::PANEL >> 4) + (kk & 3) * 2;
                     pp_mma_ss(tmem + tile * S::S_COLS, da + off, db + off, idesc_s, kk ? 1u : 0u);
                 }
                 pp_commit(&s_full[tile]);
-            }
-        };
-        auto values = [&](uint32_t tile, uint32_t slot, bool more, bool last) {
-            if (elected) {
-                const uint64_t db = pp_desc(r_s + slot * S::TILE, S::PANEL);
+            };
+            auto values = [&](uint32_t tile, uint32_t slot, uint32_t parity, bool more, bool last) -> bool {
+                const uint64_t db = v_desc + slot * (S::TILE >> 4);
 #pragma unroll
-                for (uint32_t kk = 0; kk < PP_KEYS / 16; kk++)
-                    pp_mma_ts(tmem + S::O_COL + tile * 128, tmem + tile * S::S_COLS + kk * 8, db + kk * (2048 >> 4), idesc_o, (more || kk) ? 1u : 0u);
+                for (uint32_t h = 0; h < 2; h++) {
+                    if (!pp_wait(&p_full[2 * tile + h], parity, gave_up)) return false;
+                    pp_after();
+#pragma unroll
+                    for (uint32_t kk = h * 4; kk < h * 4 + 4; kk++)
+                        pp_mma_ts(tmem + S::O_COL + tile * 128, tmem + tile * S::S_COLS + kk * 8, db + kk * (2048 >> 4), idesc_o, (more || kk) ? 1u : 0u);
+                }
                 if (last) pp_commit(&o_full[tile]);
+                return true;
+            };
+            uint32_t st = 0, par = 0;  // the ring's next tile, in the order they were loaded
+            auto next = [&](uint32_t& slot) -> bool {
+                slot = st;
+                const bool got = pp_wait(&full[st], par, gave_up);
+                if (++st == S::STAGES) {
+                    st = 0;
+                    par ^= 1;
+                }
+                return got;
+            };
+            // the last tile of V: the rows behind the last key that is seen are zeroed by the next warp
+            auto next_value = [&](uint32_t i, uint32_t& slot) -> bool {
+                if (i + 1 == n && see < (t0 + n) * PP_KEYS && !pp_wait(cleaned, 0, gave_up)) return false;
+                return next(slot);
+            };
+            bool ok = pp_wait(q_full, 0, gave_up);
+            uint32_t k_slot = 0, v_slot = 0;
+            if (!dual) {
+                ok = ok && next(k_slot);
+                pp_after();
+                if (ok) {
+                    scores(0, 0, k_slot);
+                    scores(1, 1, k_slot);
+                    pp_commit(&empty[k_slot]);
+                }
+                for (uint32_t i = 0; i < n && ok; i++) {
+                    const bool last = i + 1 == n;
+                    if (!(ok = next_value(i, v_slot))) break;
+                    if (!last && !(ok = next(k_slot))) break;
+#pragma unroll
+                    for (uint32_t tile = 0; tile < 2; tile++) {
+                        if (!(ok = values(tile, v_slot, i & 1, i > 0, last))) break;
+                        if (tile == 1) pp_commit(&empty[v_slot]);
+                        if (!last) scores(tile, tile, k_slot);
+                    }
+                    if (ok && !last) pp_commit(&empty[k_slot]);
+                }
+            } else {
+                for (uint32_t i = 0; i < 2 && i < n && ok; i++) {
+                    if (!(ok = next(k_slot))) break;
+                    pp_after();
+                    scores(i, 0, k_slot);
+                    pp_commit(&empty[k_slot]);
+                }
+                for (uint32_t i = 0; i < n && ok; i++) {
+                    const uint32_t tile = i & 1;
+                    if (!(ok = next_value(i, v_slot))) break;
+                    if (i + 2 < n && !(ok = next(k_slot))) break;
+                    if (!(ok = values(tile, v_slot, (i >> 1) & 1, i > 1, i + 2 >= n))) break;
+                    pp_commit(&empty[v_slot]);
+                    if (i + 2 < n) {
+                        scores(tile, 0, k_slot);
+                        pp_commit(&empty[k_slot]);
+                    }
+                }
             }
-        };
-        uint32_t count = 0;  // tiles taken from the ring, in the order they were loaded
-        auto next = [&](uint32_t& slot) -> bool {
-            slot = count % S::STAGES;
-            const bool got = pp_wait(&full[slot], (count / S::STAGES) & 1, gave_up);
-            count++;
-            return got;
-        };
-        // the last tile's rows of V behind the last key that is seen: zeros (their weights are zero, but a page may hold
-        // anything there, and 0 * NaN is NaN)
-        auto clean = [&](uint32_t t, uint32_t slot) {
-            const uint32_t valid = see - t * PP_KEYS;
-            if (valid >= PP_KEYS) return;
+            if (!ok) {  // given up: the products in flight read shared memory and TMEM
+                pp_commit(drained);
+                pp_land(drained, 0);
+            }
+        }
+      } else if (warp == 10 && n && see < t1 * PP_KEYS) {
+        // ---- the last tile's rows of V behind the last key that is seen: zeros (their weights are zero, but a page may
+        // hold anything there, and 0 * NaN is NaN).  In the order of the loads V of the last tile comes last.
+        const uint32_t at = 2 * n - 1, slot = at % S::STAGES, valid = see - (t1 - 1) * PP_KEYS;
+        if (pp_wait(&full[slot], (at / S::STAGES) & 1, gave_up)) {
             for (uint32_t i = valid * 8 + lane; i < PP_KEYS * 8; i += 32)
 #pragma unroll
                 for (uint32_t p = 0; p < HD / 64; p++) *reinterpret_cast<uint4*>(sR + slot * S::TILE + p * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-        };
-        bool ok = pp_wait(q_full, 0, gave_up);
-        uint32_t k_slot = 0, v_slot = 0;
-        if (!dual) {
-            ok = ok && next(k_slot);
-            pp_after();
-            if (ok) {
-                scores(0, 0, k_slot);
-                scores(1, 1, k_slot);
-                if (elected) pp_commit(&empty[k_slot]);
-            }
-            for (uint32_t i = 0; i < n && ok; i++) {
-                const bool last = i + 1 == n;
-                if (!(ok = next(v_slot))) break;
-                if (last) clean(t0 + i, v_slot);
-                if (!last && !(ok = next(k_slot))) break;
-                for (uint32_t tile = 0; tile < 2; tile++) {
-                    if (!(ok = pp_wait(&p_full[tile], i & 1, gave_up))) break;
-                    pp_after();
-                    values(tile, v_slot, i > 0, last);
-                    if (tile == 1 && elected) pp_commit(&empty[v_slot]);
-                    if (!last) scores(tile, tile, k_slot);
-                }
-                if (ok && !last && elected) pp_commit(&empty[k_slot]);
-            }
-        } else {
-            for (uint32_t i = 0; i < 2 && i < n && ok; i++) {
-                if (!(ok = next(k_slot))) break;
-                pp_after();
-                scores(i, 0, k_slot);
-                if (elected) pp_commit(&empty[k_slot]);
-            }
-            for (uint32_t i = 0; i < n && ok; i++) {
-                const uint32_t tile = i & 1;
-                if (!(ok = next(v_slot))) break;
-                if (i + 1 == n) clean(t0 + i, v_slot);
-                if (i + 2 < n && !(ok = next(k_slot))) break;
-                if (!(ok = pp_wait(&p_full[tile], (i >> 1) & 1, gave_up))) break;
-                pp_after();
-                values(tile, v_slot, i > 1, i + 2 >= n);
-                if (elected) pp_commit(&empty[v_slot]);
-                if (i + 2 < n) {
-                    scores(tile, 0, k_slot);
-                    if (elected) pp_commit(&empty[k_slot]);
-                }
-            }
         }
-        if (!ok) {  // given up: the products in flight read shared memory and TMEM
-            if (elected) pp_commit(drained);
-            for (uint32_t k = 0; k < 4096; k++) {
-                uint32_t done;
-                asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                             : "=r"(done) : "r"(pp_smem(drained)), "r"(0) : "memory");
-                if (done) break;
-            }
-        }
+        __syncwarp();
+        if (lane == 0) pp_arrive(cleaned);
       }
     }
     pp_before();
