@@ -172,8 +172,7 @@ struct PpArgs {
     float* parts_ml;
 };
 
-__device__ __forceinline__ uint32_t pp_blocks(const PpArgs& a, uint32_t b) {
-    const PgSeq s = pg_seq(a.g, b);
+__device__ __forceinline__ uint32_t pp_blocks(const PpArgs& a, const PgSeq& s) {
     const uint32_t rows = s.q_len * a.g.group;
     return rows < a.min_rows ? 0 : (rows + PP_BLOCK - 1) / PP_BLOCK;
 }
@@ -201,44 +200,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     const PgArgs& a = pa.g;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    // ---- which unit: blocks of all sequences, each sequence's last (longest) block first ----
-    __shared__ uint32_t s_seq, s_before, s_sum[PP_THREADS / 32];
-    const uint32_t seqs = a.shared ? 1 : a.batch, want = blockIdx.x / (a.kv_heads * pa.splits);
-    if (tid == 0) s_seq = 0xFFFFFFFFu;
-    uint32_t before = 0;
-    for (uint32_t b0 = 0; b0 < seqs; b0 += PP_THREADS) {
-        const uint32_t b = b0 + tid, n = b < seqs ? pp_blocks(pa, b) : 0;
-        uint32_t incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-            if (lane >= (uint32_t)o) incl += t;
-        }
-        __syncthreads();
-        if (lane == 31) s_sum[warp] = incl;
-        __syncthreads();
-        uint32_t excl = before + incl - n;
-        for (uint32_t i = 0; i < PP_THREADS / 32; i++) {
-            if (i < warp) excl += s_sum[i];
-            before += s_sum[i];
-        }
-        if (excl <= want && want < excl + n) {
-            s_seq = b;
-            s_before = excl + n;
-        }
-        __syncthreads();
-        if (s_seq != 0xFFFFFFFFu) break;
-    }
-    if (s_seq == 0xFFFFFFFFu) return;  // the grid is an upper bound (the same for all threads)
-    const uint32_t b = s_seq, block = s_before - 1 - want;
-    const uint32_t kvh = blockIdx.x / pa.splits % a.kv_heads, split = blockIdx.x % pa.splits;
-    const PgSeq sq = pg_seq(a, b);
-    const uint32_t all_rows = sq.q_len * a.group, row0 = block * PP_BLOCK, rows = min(PP_BLOCK, all_rows - row0);
-    const uint32_t see = pg_limit(sq, (row0 + rows - 1) / a.group);  // keys the block's last token sees (the most)
-    const uint32_t n_all = (see + PP_KEYS - 1) / PP_KEYS;
-    const uint32_t t0 = (uint32_t)((uint64_t)n_all * split / pa.splits), t1 = (uint32_t)((uint64_t)n_all * (split + 1) / pa.splits), n = t1 - t0;
-    const bool dual = rows <= PP_ROWS;
-
+    // ---- barriers and TMEM (while the lengths travel) ----
     if (tid == 0) {
         for (uint32_t i = 0; i < S::STAGES; i++) {
             pp_init(&full[i], 1);
@@ -260,43 +222,87 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pp_smem(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    pp_before();
-    __syncthreads();
+    pp_before();  // (the barriers of the scan publish all this)
+    // ---- which unit: blocks of all sequences, each sequence's last (longest) block first ----
+    __shared__ uint32_t s_seq, s_before, s_sum[PP_THREADS / 32];
+    __shared__ PgSeq s_found;
+    const uint32_t seqs = a.shared ? 1 : a.batch, want = blockIdx.x / (a.kv_heads * pa.splits);
+    if (tid == 0) s_seq = 0xFFFFFFFFu;
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < seqs; b0 += PP_THREADS) {
+        const uint32_t b = b0 + tid;
+        PgSeq mine = {};
+        if (b < seqs) mine = pg_seq(a, b);
+        const uint32_t n = b < seqs ? pp_blocks(pa, mine) : 0;
+        uint32_t incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            if (lane >= (uint32_t)o) incl += t;
+        }
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        uint32_t excl = before + incl - n;
+        for (uint32_t i = 0; i < PP_THREADS / 32; i++) {
+            if (i < warp) excl += s_sum[i];
+            before += s_sum[i];
+        }
+        if (excl <= want && want < excl + n) {
+            s_seq = b;
+            s_before = excl + n;
+            s_found = mine;
+        }
+        __syncthreads();
+        if (s_seq != 0xFFFFFFFFu) break;
+    }
+    if (s_seq == 0xFFFFFFFFu) {  // the grid is an upper bound (the same for all threads)
+        if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0));
+        return;
+    }
     pp_after();
+    const uint32_t b = s_seq, block = s_before - 1 - want;
+    const uint32_t kvh = blockIdx.x / pa.splits % a.kv_heads, split = blockIdx.x % pa.splits;
+    const PgSeq sq = s_found;
+    const uint32_t all_rows = sq.q_len * a.group, row0 = block * PP_BLOCK, rows = min(PP_BLOCK, all_rows - row0);
+    const uint32_t see = pg_limit(sq, (row0 + rows - 1) / a.group);  // keys the block's last token sees (the most)
+    const uint32_t n_all = (see + PP_KEYS - 1) / PP_KEYS;
+    const uint32_t t0 = (uint32_t)((uint64_t)n_all * split / pa.splits), t1 = (uint32_t)((uint64_t)n_all * (split + 1) / pa.splits), n = t1 - t0;
+    const bool dual = rows <= PP_ROWS;
+
+    // ---- Q to shared memory (all of it in flight at once; rows past the last one are zeros) ----
+    if (warp < 8 && (!dual || warp < 4)) {
+        constexpr uint32_t CH = HD / 8, STEP = 128 / CH;
+        const uint32_t w = warp >> 2, wt = tid & 127, ch = wt % CH, first = w * PP_ROWS, t_rows = min(PP_ROWS, rows - first);
+        const uint32_t whole = STEP / a.group, rest = STEP % a.group;
+        uint32_t token = (row0 + first + wt / CH) / a.group, sub = (row0 + first + wt / CH) % a.group;
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (uint64_t)sq.q0 * a.q_stride + (uint64_t)kvh * a.group * HD + ch * 8;
+        const uint32_t dst = pp_smem(sQ) + w * S::TILE + (ch >> 3) * S::PANEL;
+#pragma unroll
+        for (uint32_t qr = wt / CH; qr < PP_ROWS; qr += STEP) {
+            const bool there = qr < t_rows;
+            const uint16_t* from = there ? src + (uint64_t)token * a.q_stride + (uint64_t)sub * HD : src;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)), "l"(from), "r"(there ? 16u : 0u) : "memory");
+            token += whole;
+            sub += rest;
+            if (sub >= a.group) {
+                sub -= a.group;
+                token++;
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     // all 512 columns are this CTA's, so they start at 0; a constant keeps the products' addresses in uniform registers
     constexpr uint32_t tmem = 0;
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PP_MORE));
         // ---- softmax and epilogue: warpgroup w owns tile w (or, where the block is one tile, its keys' odd tiles) ----
-        const uint32_t w = warp >> 2, r = (warp & 3) * 32 + lane, wt = tid & 127;
+        const uint32_t w = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t first = dual ? 0 : w * PP_ROWS;  // the tile's first row of the block
         const uint32_t t_rows = min(PP_ROWS, rows - first);
-        // Q rows to shared memory (rows past the last one are zeros)
-        if (!dual || w == 0) {
-            // (eight rows' loads in flight per thread: one at a time costs a memory latency each, 13 us per unit)
-            constexpr uint32_t CH = HD / 8, STEP = 128 / CH, U = 8;
-            const uint32_t c = wt % CH;
-#pragma unroll 1
-            for (uint32_t i0 = wt / CH; i0 < PP_ROWS; i0 += STEP * U) {
-                uint4 v[U];
-#pragma unroll
-                for (uint32_t u = 0; u < U; u++) {
-                    const uint32_t qr = i0 + u * STEP;
-                    v[u] = make_uint4(0, 0, 0, 0);
-                    if (qr < t_rows) {
-                        const uint32_t row = row0 + first + qr, token = row / a.group, head = kvh * a.group + row % a.group;
-                        v[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + token) * a.q_stride + (uint64_t)head * HD + c * 8);
-                    }
-                }
-#pragma unroll
-                for (uint32_t u = 0; u < U; u++) {
-                    const uint32_t qr = i0 + u * STEP;
-                    *reinterpret_cast<uint4*>(sQ + w * S::TILE + (c >> 3) * S::PANEL + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[u];
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) pp_arrive(q_full);
 
@@ -462,36 +468,100 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 l = fmaf(l, f, other[HD * 128 + 128 + r] * g);
                 ml = M;
             }
-            const uint64_t grow = (uint64_t)(sq.q0 + token) * a.group * a.kv_heads + head, all = (uint64_t)a.tokens * a.group * a.kv_heads;
-            const bool store = r < t_rows;
+            // A thread holds a row, memory wants rows side by side: they go through the warp's share of its Q tile (every
+            // product that reads it is complete).  (Stored from the row's own thread, 8 bytes in each of 32 lines an
+            // instruction, a unit's output took 7 us.)
+            const uint32_t heads = a.group * a.kv_heads, grow = (sq.q0 + token) * heads + head;
+            const uint64_t all = (uint64_t)a.tokens * heads;
             PgEnd e = {};
-            float* part = nullptr;
-            if (store) {
-                if (pa.splits > 1) {
-                    part = pa.parts_acc + ((uint64_t)split * all + grow) * HD;
-                    *reinterpret_cast<float2*>(pa.parts_ml + ((uint64_t)split * all + grow) * 2) = make_float2(ml, l);
-                } else {
-                    e = pg_end(a, sq.q0 + token, head, ml, l, true);
-                }
+            e.f = 1.0f;
+            if (r < t_rows) {
+                if (pa.splits > 1) *reinterpret_cast<float2*>(pa.parts_ml + (split * all + grow) * 2) = make_float2(ml, l);
+                else e = pg_end(a, sq.q0 + token, head, ml, l, true);
             }
-#pragma unroll 1
-            for (uint32_t i = 0; i < HD; i += 32) {
-                float o[32];
+            uint8_t* stage = sQ + w * S::TILE + (warp & 3) * (S::TILE / 4);
+            const uint32_t n_rows = t_rows > (warp & 3) * 32 ? min(32u, t_rows - (warp & 3) * 32) : 0;
+            auto columns = [&](uint32_t from, float (&o)[32]) {  // 32 of the row's columns
                 if (it) {
-                    pp_tmem_ld32(t_o + i, o);
+                    pp_tmem_ld32(t_o + from, o);
                     pp_ld_done();
-                }
+                } else {
 #pragma unroll
-                for (uint32_t k = 0; k < 32; k++) {
-                    if (!it) o[k] = 0.0f;
-                    if (join) o[k] = fmaf(o[k], f, other[(i + k) * 128 + r] * g);
+                    for (uint32_t i = 0; i < 32; i++) o[i] = 0.0f;
                 }
-                if (store) {
+                if (join) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 32; k += 4) {
-                        const float4 v = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                        if (part) *reinterpret_cast<float4*>(part + i + k) = v;
-                        else pg_store4<T, HD>(a, e, i + k, v);
+                    for (uint32_t i = 0; i < 32; i++) o[i] = fmaf(o[i], f, other[(from + i) * 128 + r] * g);
+                }
+            };
+            if (pa.splits == 1 && !a.rows_acc && !a.base_acc) {
+                // the call's output: whole rows in its type, 16 bytes a thread
+                constexpr uint32_t PER = HD / 8, N = PER;  // threads of a row; rows of each thread (32 * PER / 32)
+                const uint32_t row_in = lane / PER, piece = lane % PER;
+#pragma unroll 1
+                for (uint32_t h = 0; h < HD; h += 32) {
+                    float o[32];
+                    columns(h, o);
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) {
+                        uint4 v;
+                        v.x = PgType<T>::pack(o[8 * i] * e.f, o[8 * i + 1] * e.f);
+                        v.y = PgType<T>::pack(o[8 * i + 2] * e.f, o[8 * i + 3] * e.f);
+                        v.z = PgType<T>::pack(o[8 * i + 4] * e.f, o[8 * i + 5] * e.f);
+                        v.w = PgType<T>::pack(o[8 * i + 6] * e.f, o[8 * i + 7] * e.f);
+                        *reinterpret_cast<uint4*>(stage + lane * (HD * 2) + (((h / 8 + i) ^ (lane & 7)) << 4)) = v;
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (uint32_t i0 = 0; i0 < N; i0 += 8) {
+                    uint4 v[8];
+                    uint32_t to[8];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++) {
+                        const uint32_t k = (i0 + i) * (32 / PER) + row_in;
+                        v[i] = *reinterpret_cast<const uint4*>(stage + k * (HD * 2) + ((piece ^ (k & 7)) << 4));
+                        to[i] = __shfl_sync(0xFFFFFFFFu, grow, k);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++)
+                        if ((i0 + i) * (32 / PER) + row_in < n_rows) *reinterpret_cast<uint4*>(a.out + (uint64_t)to[i] * HD + piece * 8) = v[i];
+                }
+            } else {
+                // partial results and rows that are joined: 32 bits, half of the columns at a time
+                constexpr uint32_t COLS = HD / 2, PER = COLS / 4, N = PER;
+                const uint32_t row_in = lane / PER, piece = lane % PER;
+#pragma unroll 1
+                for (uint32_t h = 0; h < 2; h++) {
+                    __syncwarp();
+#pragma unroll 1
+                    for (uint32_t c0 = 0; c0 < COLS; c0 += 32) {
+                        float o[32];
+                        columns(h * COLS + c0, o);
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; i++)
+                            *reinterpret_cast<float4*>(stage + lane * (COLS * 4) + (((c0 / 4 + i) ^ (lane & 7)) << 4)) =
+                                make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                    __syncwarp();
+#pragma unroll 1
+                    for (uint32_t i0 = 0; i0 < N; i0 += 8) {
+                        float4 v[8];
+                        PgEnd ek[8];
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; i++) {
+                            const uint32_t k = (i0 + i) * (32 / PER) + row_in;
+                            v[i] = *reinterpret_cast<const float4*>(stage + k * (COLS * 4) + ((piece ^ (k & 7)) << 4));
+                            ek[i].f = __shfl_sync(0xFFFFFFFFu, e.f, k);
+                            ek[i].g = __shfl_sync(0xFFFFFFFFu, e.g, k);
+                            ek[i].row = __shfl_sync(0xFFFFFFFFu, grow, k);
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; i++) {
+                            if ((i0 + i) * (32 / PER) + row_in >= n_rows) continue;
+                            if (pa.splits > 1) *reinterpret_cast<float4*>(pa.parts_acc + (split * all + ek[i].row) * HD + h * COLS + piece * 4) = v[i];
+                            else pg_store4<T, HD>(a, ek[i], h * COLS + piece * 4, v[i]);
+                        }
                     }
                 }
             }
