@@ -180,6 +180,8 @@ static qb200_status pg_check_cache(const char* who, const qb200_paged_kv* kv, co
     if (b->table_width == 0 || b->table_stride < b->table_width) return fail(QB200_ERR_LENGTH, w + ": table rows overlap or are empty");
     if ((uint64_t)b->table_width * ps > 0x7FFFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, w + ": a table row holds 2^31 keys or more");
     if (tokens > 0x7FFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, w + ": more than 2^27 new tokens");
+    if ((uint64_t)b->batch * kv->kv_heads * (((uint64_t)b->table_width * ps + 63) / 64) > 0xFFFFFFFFull)
+        return fail(QB200_ERR_NOT_SUPPORTED, w + ": the table spans 2^32 tiles of 64 keys or more");
     if (!b->cu_q && tokens != b->batch)
         return fail(QB200_ERR_LENGTH, w + ": without cu_q every sequence has one new token: " + std::to_string(tokens) + " tokens for " +
                                           std::to_string(b->batch) + " sequences");
@@ -384,7 +386,9 @@ qb200_status qb200_paged_attention(const qb200_paged_kv* kv, const qb200_paged_b
     return pg_phase(a, kv->dtype, kv->head_dim, sms, scratch, static_cast<cudaStream_t>(stream));
 }
 
-// The prefix phase leaves (m, l, acc) of every row in 32 bits; the phase over the sequences' own keys joins them.
+// The prefix phase leaves the state (m, l, acc) of every row in 32 bits; the phase over the sequences' own keys joins it
+// as it writes the row.  (Joining the ranges of the prefix there too, instead of in a kernel of their own, put 18
+// dependent reads behind every unit: 95 us instead of 63 for 64 sequences behind 8192 keys.)
 static PgArgs prefix_args(const PgArgs& own, const int32_t* pages, uint64_t prefix_len, uint32_t hd, float* rows) {
     PgArgs a = own;
     a.shared = (uint32_t)prefix_len;

@@ -39,12 +39,12 @@ struct PgArgs {
     uint32_t shared;            // keys of a shared prefix: all tokens of the batch are one sequence that sees keys [0, shared)
     float score_mul;            // log2 e * scale without a cap; scale / cap with one
     float cap_mul;              // cap * log2 e, 0: no cap
-    // results: rows of `out` [tokens, heads * hd] joined with `base` where given, or rows of `rows_out`
+    // results: rows of `out` [tokens, heads * hd], joined with the state that a first phase left of every row
     uint16_t* out;
     float* lse;                 // [tokens, heads] or null
-    const float* base_acc;      // [tokens, heads, hd] and [tokens, heads, 2] (m, l): what a first phase left
+    const float* base_acc;      // [tokens * heads][hd] and [tokens * heads][2] (m, l), or null
     const float* base_ml;
-    float* rows_acc;            // the same two, written instead of out by the first phase
+    float* rows_acc;            // the same two, written instead of out by a first phase
     float* rows_ml;
     float* parts;               // partial results of units that several CTAs share
     int32_t* meta;
@@ -157,20 +157,17 @@ __device__ __forceinline__ float pg_weight(float m, float M) { return m == -INFI
 // The end of one row's state (m, l): joined with what an earlier phase left and normalised, or kept for a later phase.
 // acc goes through pg_store4, four columns at a time.
 struct PgEnd {
-    float f, g;    // factors of this state's and the earlier phase's acc; 1 / l is in both
-    uint64_t row;
+    float f, g;  // factors of this state's acc and of the earlier phase's (1 / l is in both)
+    uint32_t row;
 };
 __device__ __forceinline__ PgEnd pg_end(const PgArgs& a, uint32_t token, uint32_t head, float m, float l, bool first) {
-    PgEnd e;
-    e.row = (uint64_t)token * a.group * a.kv_heads + head;
-    e.f = 1.0f;
-    e.g = 0.0f;
+    PgEnd e = {1.0f, 0.0f, token * a.group * a.kv_heads + head};
     if (a.rows_acc) {
-        if (first) *reinterpret_cast<float2*>(a.rows_ml + e.row * 2) = make_float2(m, l);
+        if (first) *reinterpret_cast<float2*>(a.rows_ml + (uint64_t)e.row * 2) = make_float2(m, l);
         return e;
     }
     if (a.base_acc) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.base_ml + e.row * 2);
+        const float2 ml = *(reinterpret_cast<const float2*>(a.base_ml) + e.row);
         const float M = fmaxf(m, ml.x);
         e.f = pg_weight(m, M);
         e.g = pg_weight(ml.x, M);
@@ -186,7 +183,7 @@ __device__ __forceinline__ PgEnd pg_end(const PgArgs& a, uint32_t token, uint32_
 template <typename T, uint32_t HD>
 __device__ __forceinline__ void pg_store4(const PgArgs& a, const PgEnd& e, uint32_t col, float4 v) {
     if (a.rows_acc) {
-        *reinterpret_cast<float4*>(a.rows_acc + e.row * HD + col) = v;
+        *reinterpret_cast<float4*>(a.rows_acc + (uint64_t)e.row * HD + col) = v;
         return;
     }
     v.x *= e.f;
@@ -194,7 +191,7 @@ __device__ __forceinline__ void pg_store4(const PgArgs& a, const PgEnd& e, uint3
     v.z *= e.f;
     v.w *= e.f;
     if (a.base_acc) {
-        const float4 w = *reinterpret_cast<const float4*>(a.base_acc + e.row * HD + col);
+        const float4 w = *reinterpret_cast<const float4*>(a.base_acc + (uint64_t)e.row * HD + col);
         v.x = fmaf(w.x, e.g, v.x);
         v.y = fmaf(w.y, e.g, v.y);
         v.z = fmaf(w.z, e.g, v.z);
@@ -203,7 +200,7 @@ __device__ __forceinline__ void pg_store4(const PgArgs& a, const PgEnd& e, uint3
     uint2 o;
     o.x = PgType<T>::pack(v.x, v.y);
     o.y = PgType<T>::pack(v.z, v.w);
-    *reinterpret_cast<uint2*>(a.out + e.row * HD + col) = o;
+    *reinterpret_cast<uint2*>(a.out + (uint64_t)e.row * HD + col) = o;
 }
 template <typename T, uint32_t HD>
 __device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_t head, uint32_t col, float m, float l, float4 v) {
@@ -211,6 +208,7 @@ __device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_
 }
 
 // Attention over packed rows (paged_rows.cu): grid of CTAs and floats of partial results it may use.
+uint64_t pg_rows_most_tiles(const PgArgs& a);  // below 2^32, or the call is refused
 uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms);
 uint64_t pg_rows_part_floats(uint32_t grid, uint32_t hd);
 qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t grid, cudaStream_t st);

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     const uint32_t all_rows = sq.q_len * a.group, row0 = block * PP_BLOCK, rows = min(PP_BLOCK, all_rows - row0);
     const uint32_t see = pg_limit(sq, (row0 + rows - 1) / a.group);  // keys the block's last token sees (the most)
     const uint32_t n_all = (see + PP_KEYS - 1) / PP_KEYS;
-    const uint32_t t0 = (uint32_t)((uint64_t)n_all * split / pa.splits), t1 = (uint32_t)((uint64_t)n_all * (split + 1) / pa.splits), n = t1 - t0;
+    const uint32_t t0 = n_all * split / pa.splits, t1 = n_all * (split + 1) / pa.splits, n = t1 - t0;  // (below 2^24 tiles, at most 148 splits)
     const bool dual = rows <= PP_ROWS;
 
     // ---- Q to shared memory (all of it in flight at once; rows past the last one are zeros) ----
@@ -473,10 +473,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             // instruction, a unit's output took 7 us.)
             const uint32_t heads = a.group * a.kv_heads, grow = (sq.q0 + token) * heads + head;
             const uint64_t all = (uint64_t)a.tokens * heads;
+            const bool parts = pa.splits > 1;
             PgEnd e = {};
-            e.f = 1.0f;
             if (r < t_rows) {
-                if (pa.splits > 1) *reinterpret_cast<float2*>(pa.parts_ml + (split * all + grow) * 2) = make_float2(ml, l);
+                if (parts) *reinterpret_cast<float2*>(pa.parts_ml + (split * all + grow) * 2) = make_float2(ml, l);
                 else e = pg_end(a, sq.q0 + token, head, ml, l, true);
             }
             uint8_t* stage = sQ + w * S::TILE + (warp & 3) * (S::TILE / 4);
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     for (uint32_t i = 0; i < 32; i++) o[i] = fmaf(o[i], f, other[(from + i) * 128 + r] * g);
                 }
             };
-            if (pa.splits == 1 && !a.rows_acc && !a.base_acc) {
+            if (!parts && !a.rows_acc && !a.base_acc) {
                 // the call's output: whole rows in its type, 16 bytes a thread
                 constexpr uint32_t PER = HD / 8, N = PER;  // threads of a row; rows of each thread (32 * PER / 32)
                 const uint32_t row_in = lane / PER, piece = lane % PER;
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
 #pragma unroll
                         for (uint32_t i = 0; i < 8; i++) {
                             if ((i0 + i) * (32 / PER) + row_in >= n_rows) continue;
-                            if (pa.splits > 1) *reinterpret_cast<float4*>(pa.parts_acc + (split * all + ek[i].row) * HD + h * COLS + piece * 4) = v[i];
+                            if (parts) *reinterpret_cast<float4*>(pa.parts_acc + (split * all + ek[i].row) * HD + h * COLS + piece * 4) = v[i];
                             else pg_store4<T, HD>(a, ek[i], h * COLS + piece * 4, v[i]);
                         }
                     }

@@ -7,10 +7,10 @@
 //
 // A CTA has four warps and each takes 16 of a tile's keys on its own: its K and V rows travel by 16-byte asynchronous
 // copies through a ring of its own (no barrier in the loop), S = Q K^T and O += P V run on the tensor pipe
-// (m16n8k16; the packed rows are the 16) and the softmax is one pass with a running maximum.  The warps' results are
-// joined once per unit.  P is rounded to the cache's type for the second product (half a step, 2^-8 in bf16, of each
-// weight, while l adds the unrounded weights): the errors are independent across keys and stay below the rounding of
-// the output itself.
+// (m16n8k16; the packed rows are the 16) and the softmax is one pass with a running maximum.  The ring runs on across
+// units: while one unit's warps are joined and its rows written, the next one's keys are already under way.
+// P is rounded to the cache's type for the second product (half a step, 2^-8 in bf16, of each weight, while l adds
+// the unrounded weights): the errors are independent across keys and stay below the rounding of the output itself.
 #include <string>
 
 #include "paged.cuh"
@@ -21,10 +21,12 @@ constexpr uint32_t PR_WARPS = 4, PR_KEYS = 16, PR_TILE = PR_WARPS * PR_KEYS, PR_
 static_assert(PR_ROWS == 16, "the rows of one tensor instruction");
 template <uint32_t HD> struct PrShape {
     static constexpr uint32_t ROW = HD * 2, STAGE = 2 * PR_KEYS * ROW;  // bytes of a row; of a stage (K, then V)
-    static constexpr uint32_t STAGES = HD == 128 ? 3 : 6, WARP = STAGES * STAGE, SMEM = PR_WARPS * WARP;
-    static constexpr uint32_t ACC = HD + 8;  // floats between rows of the joined accumulator (no bank conflicts)
+    static constexpr uint32_t STAGES = HD == 128 ? 3 : 6, WARP = STAGES * STAGE, RING = PR_WARPS * WARP;
+    static constexpr uint32_t PASS = 4, ACC = HD + 4;  // rows that the warps join at a time, floats between them (no bank conflicts)
+    static constexpr uint32_t JOIN = RING, ML = JOIN + PR_WARPS * PASS * ACC * 4, Q = ML + PR_WARPS * 2 * PR_ROWS * 4;
+    static constexpr uint32_t SMEM = Q + PR_ROWS * ROW;
     static constexpr uint32_t PART = PR_ROWS * (HD + 2);  // floats of one partial result: m, l [16] each, acc [16][hd]
-    static_assert(PR_ROWS * ACC * 4 + 2 * PR_ROWS * 4 <= WARP, "a warp's results fit its ring");
+    static_assert(2 * (SMEM + 4096) <= 228 * 1024, "two CTAs per SM");
 };
 
 __device__ __forceinline__ uint32_t pr_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -50,174 +52,223 @@ __device__ __forceinline__ void pr_mma(float (&d)[4], const uint32_t (&a)[4], ui
 }
 
 // Tiles of one unit of a sequence (a unit without keys still has one: it writes zeros), and of all its units; none
-// where the sequence has more rows than a unit holds (the prompt kernel takes those) or none.
-__device__ __forceinline__ uint32_t pr_tiles(const PgSeq& s) { return max(1u, (s.see + PR_TILE - 1) / PR_TILE); }
-__device__ __forceinline__ uint64_t pr_weight(const PgArgs& a, const PgSeq& s) {
+// where the sequence has more rows than a unit holds (the prompt kernel takes those) or none.  The host has made sure
+// that all tiles of a call are fewer than 2^32.
+__device__ __forceinline__ uint32_t pr_tiles(const PgSeq& s) { return max(1u, (s.kv + PR_TILE - 1) / PR_TILE); }
+__device__ __forceinline__ uint32_t pr_weight(const PgArgs& a, const PgSeq& s) {
     const uint64_t rows = (uint64_t)s.q_len * a.group;
-    return rows == 0 || rows > PG_FEW_ROWS ? 0 : (uint64_t)a.kv_heads * pr_tiles(s);
+    return rows == 0 || rows > PG_FEW_ROWS ? 0 : a.kv_heads * pr_tiles(s);
 }
 
-// Where the CTA's run of tiles lies: [run0, run1) of the total, and the sequence that holds tile run0 (first: its
-// first tile).  All threads of the CTA take part.
+// Sequences whose lengths the CTA keeps in shared memory: the first ones of the call.
+constexpr uint32_t PR_KEPT = PR_WARPS * 32;
+
+// The CTA's run of tiles, [run0, run1) of the total, and the sequence that holds tile run0 (first: its first tile).
+// Runs differ by at most one tile, the longer ones first.
 struct PrRun {
-    uint64_t run0, run1, first, total;
-    uint32_t seq, ctas;  // CTAs that have a run: none of theirs is empty
+    uint32_t run0, run1, first, seq;
+    uint32_t base, extra;  // tiles of the shorter runs, how many runs are one longer
 };
-__device__ __forceinline__ PrRun pr_find_run(const PgArgs& a, uint32_t seqs) {
-    __shared__ uint64_t s_warp[PR_WARPS];
-    __shared__ uint64_t s_first;
-    __shared__ uint32_t s_seq;
+// All threads of the CTA take part; false where it has no run (the same for all).
+__device__ __forceinline__ bool pr_find_run(const PgArgs& a, uint32_t seqs, PgSeq* kept, PrRun& r) {
+    __shared__ uint32_t s_warp[PR_WARPS], s_first, s_seq;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint64_t sum = 0, mine = 0;
-    for (uint32_t b = tid; b < seqs; b += PR_WARPS * 32) sum += mine = pr_weight(a, pg_seq(a, b));
+    PgSeq mine = {};
+    uint32_t sum = 0, w0 = 0;
+    for (uint32_t b = tid; b < seqs; b += PR_KEPT) {
+        const PgSeq s = pg_seq(a, b);
+        const uint32_t w = pr_weight(a, s);
+        if (b < PR_KEPT) {
+            mine = s;
+            w0 = w;
+        }
+        sum += w;
+    }
+    kept[tid] = mine;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) s_warp[warp] = sum;
-    if (tid == 0) s_seq = seqs;
+    if (tid == 0) s_seq = 0xFFFFFFFFu;
     __syncthreads();
-    uint64_t total = 0;
+    uint32_t total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < PR_WARPS; w++) total += s_warp[w];
-    PrRun r;
-    r.total = total;
-    r.ctas = (uint32_t)min((uint64_t)gridDim.x, total);
-    r.seq = seqs;
-    r.run0 = r.run1 = r.first = 0;
-    if (blockIdx.x >= r.ctas) return r;  // the same for all threads of the CTA
-    r.run0 = total * blockIdx.x / r.ctas;
-    r.run1 = total * (blockIdx.x + 1) / r.ctas;
-    uint64_t before = 0;
-    for (uint32_t b0 = 0; b0 < seqs; b0 += PR_WARPS * 32) {
-        const uint32_t b = b0 + tid;
-        const uint64_t w = b < seqs ? (seqs <= PR_WARPS * 32 ? mine : pr_weight(a, pg_seq(a, b))) : 0;
-        uint64_t incl = w;
+    const uint32_t ctas = min(gridDim.x, total), i = blockIdx.x;
+    if (i >= ctas) return false;
+    r.base = total / ctas;
+    r.extra = total - r.base * ctas;
+    r.run0 = i * r.base + min(i, r.extra);
+    r.run1 = r.run0 + r.base + (i < r.extra ? 1 : 0);
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < seqs; b0 += PR_KEPT) {
+        const uint32_t b = b0 + tid, w = b0 == 0 ? w0 : b < seqs ? pr_weight(a, pg_seq(a, b)) : 0;
+        uint32_t incl = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
             if (lane >= (uint32_t)o) incl += t;
         }
         __syncthreads();  // s_warp is read by all before it is written again
         if (lane == 31) s_warp[warp] = incl;
         __syncthreads();
-        uint64_t excl = before + incl - w;
-        for (uint32_t i = 0; i < PR_WARPS; i++) {
-            if (i < warp) excl += s_warp[i];
-            before += s_warp[i];
+        uint32_t excl = before + incl - w;
+#pragma unroll
+        for (uint32_t k = 0; k < PR_WARPS; k++) {
+            if (k < warp) excl += s_warp[k];
+            before += s_warp[k];
         }
-        if (excl <= r.run0 && r.run0 < excl + w) {
+        if (excl <= r.run0 && r.run0 - excl < w) {
             s_seq = b;
             s_first = excl;
         }
         __syncthreads();
-        if (s_seq < seqs) break;
+        if (s_seq != 0xFFFFFFFFu) break;
     }
     r.seq = s_seq;
     r.first = s_first;
-    return r;
+    return true;
+}
+
+// A place in the CTA's run: tile t of K/V head kvh of sequence b.
+struct PrAt {
+    PgSeq s;
+    uint32_t b, kvh, t, tiles, left;  // left: tiles of the run from here on
+};
+__device__ __forceinline__ PgSeq pr_seq(const PgArgs& a, const PgSeq* kept, uint32_t b) { return b < PR_KEPT ? kept[b] : pg_seq(a, b); }
+// n tiles further (not past the unit's end).
+__device__ __forceinline__ void pr_advance(const PgArgs& a, const PgSeq* kept, PrAt& p, uint32_t n) {
+    p.left -= n;
+    p.t += n;
+    if (p.left == 0 || p.t < p.tiles) return;
+    p.t = 0;
+    if (++p.kvh < a.kv_heads) return;
+    p.kvh = 0;
+    do p.s = pr_seq(a, kept, ++p.b);  // (the run goes on, so there is one)
+    while (pr_weight(a, p.s) == 0);
+    p.tiles = pr_tiles(p.s);
 }
 
 template <typename T, uint32_t HD, bool SCORED>
-__global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a) {
+__global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_constant__ PgArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     using S = PrShape<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ PgSeq kept[PR_KEPT];
     constexpr uint32_t KS = HD / 16, NP = HD / 16, CH = HD / 8;  // k-steps of S, pairs of column tiles of O, 16-byte chunks of a row
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane >> 2, part4 = lane & 3;
-    const uint32_t seqs = a.shared ? 1 : a.batch;
-    const PrRun run = pr_find_run(a, seqs);
     int32_t* meta = a.meta + blockIdx.x * 8;
     if (tid == 0) meta[0] = -1;
-    if (run.run0 == run.run1) return;
-    uint8_t* ring = smem + warp * S::WARP;
-    const uint32_t ring_s = pr_smem(ring);
-    uint32_t b = run.seq;
-    PgSeq sq = pg_seq(a, b);
-    uint64_t seq_first = run.first, at = run.run0;
-    uint32_t slot = 0;  // the CTA's first partial unit goes to its slot 0, the last one to slot 1
-    while (at < run.run1) {
-        while (at >= seq_first + pr_weight(a, sq)) {  // on to the next sequence that has rows here
-            seq_first += pr_weight(a, sq);
-            if (++b >= seqs) return;
-            sq = pg_seq(a, b);
-        }
-        const uint32_t tiles = pr_tiles(sq), kvh = (uint32_t)((at - seq_first) / tiles);
-        const uint64_t unit_first = seq_first + (uint64_t)kvh * tiles;
-        const uint32_t t0 = (uint32_t)(at - unit_first);
-        const uint32_t t1 = (uint32_t)min((uint64_t)tiles, run.run1 - unit_first);
-        at = unit_first + t1;
-        const uint32_t rows = sq.q_len * a.group;
-        const uint32_t see = pg_limit(sq, sq.q_len - 1);  // keys the last token sees (the most)
-        const uint32_t te = min(t1, (see + PR_TILE - 1) / PR_TILE);
-        const int32_t* table = a.table + (a.shared ? 0 : (uint64_t)b * a.table_stride);
+    PrRun run;
+    if (!pr_find_run(a, a.shared ? 1 : a.batch, kept, run)) return;
+    const uint32_t ring_s = pr_smem(smem + warp * S::WARP), q_s = pr_smem(smem + S::Q);
+    float* j_acc = reinterpret_cast<float*>(smem + S::JOIN);
+    float* j_ml = reinterpret_cast<float*>(smem + S::ML);
 
-        // this thread's two rows: what they see, and the bias they get
-        uint32_t lim[2];
-        float slope[2];
-        int32_t pos[2];
-        uint32_t qf[KS][4];
-        {
-            const uint16_t* qp[2] = {nullptr, nullptr};
-#pragma unroll
-            for (uint32_t i = 0; i < 2; i++) {
-                const uint32_t r = quad + 8 * i;
-                lim[i] = 0;
-                slope[i] = 0.0f;
-                pos[i] = 0;
-                if (r < rows) {
-                    const uint32_t token = r / a.group, head = kvh * a.group + r % a.group;
-                    lim[i] = pg_limit(sq, token);
-                    qp[i] = static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + token) * a.q_stride + (uint64_t)head * HD;
-                    if (SCORED && a.slopes) {
-                        slope[i] = a.slopes[head] * PG_LOG2E;
-                        pos[i] = pg_position(a, sq, token);
-                    }
-                }
-            }
-#pragma unroll
-            for (uint32_t ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) {
-                    const uint16_t* p = qp[i & 1];
-                    qf[ks][i] = p ? *reinterpret_cast<const uint32_t*>(p + ks * 16 + (i >> 1) * 8 + part4 * 2) : 0u;
-                }
-        }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2 * NP][4];
-#pragma unroll
-        for (uint32_t n = 0; n < 2 * NP; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    PrAt here, ahead;  // what is computed and what is fetched
+    here.b = run.seq;
+    here.s = pr_seq(a, kept, run.seq);
+    here.tiles = pr_tiles(here.s);
+    here.kvh = (run.run0 - run.first) / here.tiles;
+    here.t = run.run0 - run.first - here.kvh * here.tiles;
+    here.left = run.run1 - run.run0;
+    ahead = here;
 
-        // the warp's 16 keys of tile t -> a stage of its ring (16-byte chunk c of a row at c ^ (row & 7)); keys that no
-        // row sees are zeros, whatever the page holds there, and so are all keys of a page that is not in the pool
-        auto fetch = [&](uint32_t t, uint32_t st) {
-            const uint32_t key0 = t * PR_TILE + warp * PR_KEYS;
-            uint32_t valid = key0 < see ? min(see - key0, PR_KEYS) : 0;
-            int32_t page = 0;
-            if (valid) {
-                page = table[key0 >> a.ps_log];
-                if ((uint32_t)page >= a.n_pages) {
-                    pg_report(a.status, QB200_ERR_INVALID_PARAM);
-                    page = 0;
-                    valid = 0;
-                }
+    // ---- the ring: the warp's 16 keys of one tile a stage (16-byte chunk c of a row at c ^ (row & 7)).  Keys behind the
+    // sequence's last one are zeros, whatever the page holds there, and so are all keys of a page that is not in the pool.
+    // The next tile's page number is read a step before it is needed.
+    int32_t n_page = 0;
+    uint32_t n_kvh = 0, n_key = 0, n_valid = 0;
+    bool n_there = false;
+    auto look = [&]() {
+        n_there = ahead.left != 0;
+        if (!n_there) return;
+        n_key = ahead.t * PR_TILE + warp * PR_KEYS;
+        n_valid = n_key < ahead.s.kv ? min(ahead.s.kv - n_key, PR_KEYS) : 0;
+        n_kvh = ahead.kvh;
+        if (n_valid) n_page = a.table[(a.shared ? 0 : (uint64_t)ahead.b * a.table_stride) + (n_key >> a.ps_log)];
+        pr_advance(a, kept, ahead, 1);
+    };
+    auto fetch = [&](uint32_t st) {
+        if (n_there) {
+            if (n_valid && (uint32_t)n_page >= a.n_pages) {
+                pg_report(a.status, QB200_ERR_INVALID_PARAM);
+                n_valid = 0;
             }
-            const uint64_t base = (((uint64_t)(uint32_t)page * a.kv_heads + kvh) << a.ps_log) + (key0 & ((1u << a.ps_log) - 1));
+            const uint64_t base = n_valid ? (((uint64_t)(uint32_t)n_page * a.kv_heads + n_kvh) << a.ps_log) + (n_key & ((1u << a.ps_log) - 1)) : 0;
             const uint32_t dst = ring_s + st * S::STAGE;
 #pragma unroll
             for (uint32_t i = 0; i < PR_KEYS * CH / 32; i++) {
-                const uint32_t id = i * 32 + lane, row = id / CH, c = id % CH, bytes = row < valid ? 16u : 0u;
+                const uint32_t id = i * 32 + lane, row = id / CH, c = id % CH, bytes = row < n_valid ? 16u : 0u;
                 const uint64_t src = (base + (bytes ? row : 0)) * HD + c * 8;
                 const uint32_t d = dst + row * S::ROW + ((c ^ (row & 7)) << 4);
                 pr_copy16(d, a.k + src, bytes);
                 pr_copy16(d + PR_KEYS * S::ROW, a.v + src, bytes);
             }
-        };
-#pragma unroll
-        for (uint32_t i = 0; i + 1 < S::STAGES; i++) {
-            if (t0 + i < te) fetch(t0 + i, i);
-            pr_commit();
+            look();
         }
-        uint32_t st = 0;
-        for (uint32_t t = t0; t < te; t++) {
+        pr_commit();
+    };
+
+    // ---- Q of a unit: loaded while the unit before it is joined, then through shared memory into fragments ----
+    constexpr uint32_t QN = PR_ROWS * CH / 128;  // 16-byte chunks a thread brings
+    uint4 q_in[QN];
+    auto bring_q = [&](const PrAt& p) {
+#pragma unroll
+        for (uint32_t i = 0; i < QN; i++) {
+            const uint32_t id = i * 128 + tid, r = id / CH, c = id % CH;
+            q_in[i] = make_uint4(0, 0, 0, 0);
+            if (r < p.s.q_len * a.group)
+                q_in[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(p.s.q0 + r / a.group) * a.q_stride +
+                                                          (uint64_t)(p.kvh * a.group + r % a.group) * HD + c * 8);
+        }
+    };
+
+    bring_q(here);
+    look();
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < S::STAGES; i++) fetch(i);
+    uint32_t st = 0, slot = 0;  // slot: the CTA's first unit, where it is a part, goes to its slot 0, the last one to slot 1
+    while (true) {
+        // ---- a unit ----
+#pragma unroll
+        for (uint32_t i = 0; i < QN; i++) {
+            const uint32_t id = i * 128 + tid, r = id / CH, c = id % CH;
+            *reinterpret_cast<uint4*>(smem + S::Q + r * S::ROW + ((c ^ (r & 7)) << 4)) = q_in[i];
+        }
+        __syncthreads();
+        uint32_t qf[KS][4];
+        {
+            const uint32_t r = (((lane >> 3) & 1) << 3) | (lane & 7), sub = lane >> 4;
+#pragma unroll
+            for (uint32_t ks = 0; ks < KS; ks++) pr_ldsm(q_s + r * S::ROW + (((ks * 2 + sub) ^ (r & 7)) << 4), qf[ks]);
+        }
+        const PgSeq sq = here.s;
+        const uint32_t kvh = here.kvh, rows = sq.q_len * a.group, t0 = here.t, n = min(here.tiles - t0, here.left);
+        const bool whole = n == here.tiles;
+        // this thread's two rows: what they see, and the bias they get
+        uint32_t lim[2];
+        float slope[2];
+        int32_t pos[2];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; i++) {
+            const uint32_t r = quad + 8 * i;
+            lim[i] = 0;
+            slope[i] = 0.0f;
+            pos[i] = 0;
+            if (r < rows) {
+                lim[i] = pg_limit(sq, r / a.group);
+                if (SCORED && a.slopes) {
+                    slope[i] = a.slopes[kvh * a.group + r % a.group] * PG_LOG2E;
+                    pos[i] = pg_position(a, sq, r / a.group);
+                }
+            }
+        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2 * NP][4];
+#pragma unroll
+        for (uint32_t k = 0; k < 2 * NP; k++) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.0f;
+
+        for (uint32_t t = t0; t < t0 + n; t++) {
             pr_wait<S::STAGES - 2>();
             __syncwarp();
             const uint32_t ks_s = ring_s + st * S::STAGE, vs_s = ks_s + PR_KEYS * S::ROW;
@@ -235,17 +286,17 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a)
             const uint32_t key0 = t * PR_TILE + warp * PR_KEYS + part4 * 2;
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (uint32_t n = 0; n < 2; n++)
+            for (uint32_t k = 0; k < 2; k++)
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) {
-                    const uint32_t r = i >> 1, key = key0 + n * 8 + (i & 1);
-                    float x = s[n][i] * a.score_mul;
+                    const uint32_t r = i >> 1, key = key0 + k * 8 + (i & 1);
+                    float x = s[k][i] * a.score_mul;
                     if (SCORED) {
                         if (a.cap_mul != 0.0f) x = pg_cap(x, a.cap_mul);
                         x = fmaf(-slope[r], fabsf((float)(pos[r] - (int32_t)key)), x);
                     }
                     x = key < lim[r] ? x : -INFINITY;
-                    s[n][i] = x;
+                    s[k][i] = x;
                     mx[r] = fmaxf(mx[r], x);
                 }
             float f[2], ms[2];
@@ -261,133 +312,135 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const PgArgs a)
             }
             if (__any_sync(0xFFFFFFFFu, f[0] != 1.0f || f[1] != 1.0f)) {
 #pragma unroll
-                for (uint32_t n = 0; n < 2 * NP; n++) {
-                    o[n][0] *= f[0];
-                    o[n][1] *= f[0];
-                    o[n][2] *= f[1];
-                    o[n][3] *= f[1];
+                for (uint32_t k = 0; k < 2 * NP; k++) {
+                    o[k][0] *= f[0];
+                    o[k][1] *= f[0];
+                    o[k][2] *= f[1];
+                    o[k][3] *= f[1];
                 }
             }
             uint32_t pf[4];
 #pragma unroll
-            for (uint32_t n = 0; n < 2; n++) {
+            for (uint32_t k = 0; k < 2; k++) {
                 float p[4];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) {
-                    p[i] = pg_exp2(s[n][i] - ms[i >> 1]);
+                    p[i] = pg_exp2(s[k][i] - ms[i >> 1]);
                     l[i >> 1] += p[i];
                 }
-                pf[n * 2] = PgType<T>::pack(p[0], p[1]);
-                pf[n * 2 + 1] = PgType<T>::pack(p[2], p[3]);
+                pf[k * 2] = PgType<T>::pack(p[0], p[1]);
+                pf[k * 2 + 1] = PgType<T>::pack(p[2], p[3]);
             }
             {
                 const uint32_t key = (((lane >> 3) & 1) << 3) | (lane & 7), sub = lane >> 4;
 #pragma unroll
-                for (uint32_t n = 0; n < NP; n++) {
+                for (uint32_t k = 0; k < NP; k++) {
                     uint32_t vf[4];
-                    pr_ldsm_t(vs_s + key * S::ROW + (((n * 2 + sub) ^ (key & 7)) << 4), vf);
-                    pr_mma(o[2 * n], pf, vf[0], vf[1], T());
-                    pr_mma(o[2 * n + 1], pf, vf[2], vf[3], T());
+                    pr_ldsm_t(vs_s + key * S::ROW + (((k * 2 + sub) ^ (key & 7)) << 4), vf);
+                    pr_mma(o[2 * k], pf, vf[0], vf[1], T());
+                    pr_mma(o[2 * k + 1], pf, vf[2], vf[3], T());
                 }
             }
-            __syncwarp();  // every lane is done with the stage that the next fetch overwrites
-            {
-                const uint32_t tn = t + S::STAGES - 1;
-                const uint32_t sn = st == 0 ? S::STAGES - 1 : st - 1;
-                if (tn < te) fetch(tn, sn);
-                pr_commit();
-            }
+            __syncwarp();  // every lane is done with the stage that the next fetch overwrites: the one before this
+            fetch(st == 0 ? S::STAGES - 1 : st - 1);
             if (++st == S::STAGES) st = 0;
         }
-        pr_wait<0>();
-        __syncwarp();
 
-        // join the warps: each leaves its rows in its own ring
+        // ---- its end: on to the next unit's Q, then the warps' states are joined, PASS rows at a time ----
+        const uint32_t first_tile = run.run1 - here.left;
+        pr_advance(a, kept, here, n);
+        const bool more = here.left != 0;
+        if (more) bring_q(here);
 #pragma unroll
         for (uint32_t r = 0; r < 2; r++) {
             l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
             l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
         }
-        float* w_acc = reinterpret_cast<float*>(ring);
-        float* w_ml = w_acc + PR_ROWS * S::ACC;
-#pragma unroll
-        for (uint32_t n = 0; n < 2 * NP; n++) {
-            *reinterpret_cast<float2*>(w_acc + quad * S::ACC + n * 8 + part4 * 2) = make_float2(o[n][0], o[n][1]);
-            *reinterpret_cast<float2*>(w_acc + (quad + 8) * S::ACC + n * 8 + part4 * 2) = make_float2(o[n][2], o[n][3]);
-        }
         if (part4 == 0) {
-            w_ml[quad] = m[0];
-            w_ml[quad + 8] = m[1];
-            w_ml[PR_ROWS + quad] = l[0];
-            w_ml[PR_ROWS + quad + 8] = l[1];
+            float* ml = j_ml + warp * 2 * PR_ROWS;
+            ml[quad] = m[0];
+            ml[quad + 8] = m[1];
+            ml[PR_ROWS + quad] = l[0];
+            ml[PR_ROWS + quad + 8] = l[1];
         }
-        __syncthreads();
-        const bool whole = t0 == 0 && t1 == tiles;
         float* part = a.parts + ((uint64_t)blockIdx.x * 2 + slot) * S::PART;
-        if (!whole) {
-            // a unit that starts here and goes on: this CTA's entry names what the second kernel joins
-            if (tid == 0 && t0 == 0) {
-                meta[1] = (int32_t)slot;
-                meta[2] = (int32_t)(sq.q0);
-                meta[3] = (int32_t)rows;
-                meta[4] = (int32_t)kvh;
-                // the CTA whose run holds the unit's last tile x: the largest c with total * c / ctas <= x
-                meta[0] = (int32_t)(((unit_first + tiles) * run.ctas - 1) / run.total);
-            }
+        if (!whole && t0 == 0 && tid == 0) {  // a unit that starts here and goes on: what the second kernel joins
+            const uint32_t x = first_tile + (whole ? n : pr_tiles(sq)) - 1, cut = run.extra * (run.base + 1);
+            meta[1] = (int32_t)slot;
+            meta[2] = (int32_t)sq.q0;
+            meta[3] = (int32_t)rows;
+            meta[4] = (int32_t)kvh;
+            meta[0] = (int32_t)(x < cut ? x / (run.base + 1) : run.extra + (x - cut) / run.base);  // the CTA that has its last tile
         }
         constexpr uint32_t PER = HD / 4;  // threads of a row
-        for (uint32_t r = tid / PER; r < rows; r += PR_WARPS * 32 / PER) {
-            const uint32_t col = (tid % PER) * 4;
-            float M = -INFINITY;
+        for (uint32_t p0 = 0; p0 < rows; p0 += S::PASS) {
+            if (p0) __syncthreads();  // the rows before have been read
 #pragma unroll
-            for (uint32_t w = 0; w < PR_WARPS; w++) M = fmaxf(M, reinterpret_cast<const float*>(smem + w * S::WARP)[PR_ROWS * S::ACC + r]);
-            float L = 0.0f;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t i = 0; i < 2; i++) {
+                const uint32_t r = quad + 8 * i - p0;
+                if (r < S::PASS) {
+                    float* to = j_acc + (warp * S::PASS + r) * S::ACC + part4 * 2;
 #pragma unroll
-            for (uint32_t w = 0; w < PR_WARPS; w++) {
-                const float* p = reinterpret_cast<const float*>(smem + w * S::WARP);
-                const float g = pg_weight(p[PR_ROWS * S::ACC + r], M);
-                const float4 e = *reinterpret_cast<const float4*>(p + r * S::ACC + col);
-                L = fmaf(p[PR_ROWS * S::ACC + PR_ROWS + r], g, L);
-                v.x = fmaf(e.x, g, v.x);
-                v.y = fmaf(e.y, g, v.y);
-                v.z = fmaf(e.z, g, v.z);
-                v.w = fmaf(e.w, g, v.w);
-            }
-            if (whole) {
-                pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
-            } else {
-                if (col == 0) {
-                    part[r] = M;
-                    part[PR_ROWS + r] = L;
+                    for (uint32_t k = 0; k < 2 * NP; k++) *reinterpret_cast<float2*>(to + k * 8) = make_float2(o[k][2 * i], o[k][2 * i + 1]);
                 }
-                *reinterpret_cast<float4*>(part + 2 * PR_ROWS + r * HD + col) = v;
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (uint32_t r = p0 + tid / PER; r < min(rows, p0 + S::PASS); r += PR_WARPS * 32 / PER) {
+                const uint32_t col = (tid % PER) * 4;
+                float M = -INFINITY;
+#pragma unroll
+                for (uint32_t w = 0; w < PR_WARPS; w++) M = fmaxf(M, j_ml[w * 2 * PR_ROWS + r]);
+                float L = 0.0f;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (uint32_t w = 0; w < PR_WARPS; w++) {
+                    const float g = pg_weight(j_ml[w * 2 * PR_ROWS + r], M);
+                    const float4 e = *reinterpret_cast<const float4*>(j_acc + (w * S::PASS + r - p0) * S::ACC + col);
+                    L = fmaf(j_ml[w * 2 * PR_ROWS + PR_ROWS + r], g, L);
+                    v.x = fmaf(e.x, g, v.x);
+                    v.y = fmaf(e.y, g, v.y);
+                    v.z = fmaf(e.z, g, v.z);
+                    v.w = fmaf(e.w, g, v.w);
+                }
+                if (whole) {
+                    pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
+                } else {
+                    if (col == 0) {
+                        part[r] = M;
+                        part[PR_ROWS + r] = L;
+                    }
+                    *reinterpret_cast<float4*>(part + 2 * PR_ROWS + r * HD + col) = v;
+                }
             }
         }
+        if (!more) break;
         slot = 1;
-        __syncthreads();  // the rings are free again
+        __syncthreads();  // the join area is free again
     }
+    pr_wait<0>();
 }
 
 // Joins the partial results of the unit that starts in CTA blockIdx.x's run and ends in a later one's.  A block takes
-// the rows blockIdx.y, blockIdx.y + gridDim.y, ...; LANES groups of threads take every LANES-th part of a row (one
-// sequence's keys may be cut into dozens: taken one after the other, 37 parts cost 18 us) and meet in shared memory.
+// four of its rows, from 4 * blockIdx.y on; LANES groups of threads take every LANES-th part of a row (one sequence's
+// keys may be cut into dozens: taken one after the other, 37 parts cost 18 us) and meet in shared memory.
 template <typename T, uint32_t HD>
-__global__ void __launch_bounds__(256) k_paged_rows_join(const PgArgs a) {
+__global__ void __launch_bounds__(512) k_paged_rows_join(const __grid_constant__ PgArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     using S = PrShape<HD>;
-    constexpr uint32_t PER = HD / 4, LANES = 256 / PER, U = 3;
-    __shared__ float4 s_acc[LANES][PER];
-    __shared__ float s_m[LANES], s_l[LANES];
+    constexpr uint32_t PER = HD / 4, LANES = 512 / 4 / PER, U = 4;
+    __shared__ float4 s_acc[4][LANES][PER];
+    __shared__ float s_m[4][LANES], s_l[4][LANES];
     const int4 m0 = *reinterpret_cast<const int4*>(a.meta + blockIdx.x * 8);
-    if (m0.x < 0) return;
     const uint32_t kvh = (uint32_t)a.meta[blockIdx.x * 8 + 4];
+    if (m0.x < 0) return;
     const uint32_t last = (uint32_t)m0.x, slot0 = (uint32_t)m0.y, q0 = (uint32_t)m0.z, rows = (uint32_t)m0.w;
-    const uint32_t lane = threadIdx.x / PER, col = (threadIdx.x % PER) * 4, lanes = min(LANES, last - blockIdx.x + 1);
-    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
-        float M = -INFINITY, L = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const uint32_t piece = threadIdx.x % PER, col = piece * 4, k = threadIdx.x / PER % 4, lane = threadIdx.x / (4 * PER), r = blockIdx.y * 4 + k;
+    if (blockIdx.y * 4 >= rows) return;
+    float M = -INFINITY, L = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (r < rows) {
 #pragma unroll 1
         for (uint32_t c0 = blockIdx.x + lane; c0 <= last; c0 += LANES * U) {
             float m[U], l[U];
@@ -396,53 +449,72 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(const PgArgs a) {
             for (uint32_t u = 0; u < U; u++) {
                 const uint32_t c = min(c0 + u * LANES, last);
                 const float* p = a.parts + ((uint64_t)c * 2 + (c == blockIdx.x ? slot0 : 0)) * S::PART;
-                m[u] = c0 + u * LANES <= last ? p[r] : -INFINITY;
+                m[u] = p[r];
                 l[u] = p[PR_ROWS + r];
                 e[u] = *reinterpret_cast<const float4*>(p + 2 * PR_ROWS + r * HD + col);
             }
+            float Mn = M;
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
+                if (c0 + u * LANES <= last) Mn = fmaxf(Mn, m[u]);
+            const float f = pg_weight(M, Mn);
+            M = Mn;
+            L *= f;
+            v.x *= f;
+            v.y *= f;
+            v.z *= f;
+            v.w *= f;
 #pragma unroll
             for (uint32_t u = 0; u < U; u++) {
                 if (c0 + u * LANES > last) continue;
-                const float Mn = fmaxf(M, m[u]), f = pg_weight(M, Mn), g = pg_weight(m[u], Mn);
-                L = fmaf(L, f, l[u] * g);
-                v.x = fmaf(v.x, f, e[u].x * g);
-                v.y = fmaf(v.y, f, e[u].y * g);
-                v.z = fmaf(v.z, f, e[u].z * g);
-                v.w = fmaf(v.w, f, e[u].w * g);
-                M = Mn;
+                const float g = pg_weight(m[u], M);
+                L = fmaf(l[u], g, L);
+                v.x = fmaf(e[u].x, g, v.x);
+                v.y = fmaf(e[u].y, g, v.y);
+                v.z = fmaf(e[u].z, g, v.z);
+                v.w = fmaf(e[u].w, g, v.w);
             }
         }
-        s_acc[lane][threadIdx.x % PER] = v;
-        if (col == 0) {
-            s_m[lane] = M;
-            s_l[lane] = L;
+        s_acc[k][lane][piece] = v;
+        if (piece == 0) {
+            s_m[k][lane] = M;
+            s_l[k][lane] = L;
         }
-        __syncthreads();
-        if (lane == 0) {
-            for (uint32_t i = 1; i < lanes; i++) {
-                const float mi = s_m[i], Mn = fmaxf(M, mi), f = pg_weight(M, Mn), g = pg_weight(mi, Mn);
-                const float4 e = s_acc[i][threadIdx.x % PER];
-                L = fmaf(L, f, s_l[i] * g);
-                v.x = fmaf(v.x, f, e.x * g);
-                v.y = fmaf(v.y, f, e.y * g);
-                v.z = fmaf(v.z, f, e.z * g);
-                v.w = fmaf(v.w, f, e.w * g);
-                M = Mn;
-            }
-            pg_emit<T, HD>(a, q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
-        }
-        __syncthreads();
     }
+    __syncthreads();
+    if (lane || r >= rows) return;
+    M = s_m[k][0];
+#pragma unroll
+    for (uint32_t i = 1; i < LANES; i++) M = fmaxf(M, s_m[k][i]);
+    const float f = pg_weight(s_m[k][0], M);
+    L *= f;
+    v.x *= f;
+    v.y *= f;
+    v.z *= f;
+    v.w *= f;
+#pragma unroll
+    for (uint32_t i = 1; i < LANES; i++) {
+        const float g = pg_weight(s_m[k][i], M);
+        const float4 e = s_acc[k][i][piece];
+        L = fmaf(s_l[k][i], g, L);
+        v.x = fmaf(e.x, g, v.x);
+        v.y = fmaf(e.y, g, v.y);
+        v.z = fmaf(e.z, g, v.z);
+        v.w = fmaf(e.w, g, v.w);
+    }
+    pg_emit<T, HD>(a, q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms) {
-    // two CTAs per SM, fewer where the call cannot have as many tiles
-    const uint64_t units = a.shared ? 1 : a.batch;
+uint64_t pg_rows_most_tiles(const PgArgs& a) {
     const uint64_t keys = a.shared ? a.shared : (uint64_t)a.width << a.ps_log;
-    const uint64_t most = units * a.kv_heads * (keys ? div_ceil(keys, PR_TILE) : 1);
-    return (uint32_t)(most < 2 * sms ? (most ? most : 1) : 2 * sms);
+    return (a.shared ? 1 : (uint64_t)a.batch) * a.kv_heads * div_ceil(keys, PR_TILE);
+}
+
+uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms) {
+    const uint64_t most = pg_rows_most_tiles(a);  // two CTAs per SM, fewer where the call cannot have as many tiles
+    return (uint32_t)(most < 2 * sms ? most : 2 * sms);
 }
 
 uint64_t pg_rows_part_floats(uint32_t grid, uint32_t hd) { return (uint64_t)grid * 2 * PR_ROWS * (hd + 2) + (uint64_t)grid * 8; }
@@ -458,7 +530,7 @@ static qb200_status launch_rows(const PgArgs& a, uint32_t grid, cudaStream_t st)
     }
     QB_CUDA_TRY(pg_launch(k_paged_rows<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, a));
     const uint64_t rows = a.cu_q || a.shared ? (uint64_t)a.tokens * a.group : a.group;
-    QB_CUDA_TRY(pg_launch(k_paged_rows_join<T, HD>, dim3(grid, (uint32_t)(rows < 8 ? rows : 8)), dim3(256), 0, st, a));
+    QB_CUDA_TRY(pg_launch(k_paged_rows_join<T, HD>, dim3(grid, (uint32_t)((rows < PR_ROWS ? rows : PR_ROWS) + 3) / 4), dim3(512), 0, st, a));
     return QB200_OK;
 }
 

@@ -74,6 +74,7 @@ class PagedKVCache:
         self._ref = ctypes.byref(self.c)
         self._index = k.device.index if k.is_cuda else -1
         self._scale = 1.0 / math.sqrt(head_dim)
+        self._f32 = torch.empty(0, dtype=torch.float32, device=k.device)  # new_empty of a tensor is the quickest allocation
 
     def check(self) -> None:
         """Waits for the current stream and raises what a kernel recorded (once)."""
@@ -117,17 +118,19 @@ def _run(cache: PagedKVCache, fn, *args) -> None:
 
 def _rows(x: torch.Tensor, heads: int, cache: PagedKVCache, what: str) -> Tuple[int, int, int]:
     """(tokens, heads, row stride) of x ``[tokens, heads * head_dim]`` with contiguous columns; heads = 0: as many as there are."""
-    hd, shape = cache.head_dim, x.shape
-    if len(shape) != 2 or shape[1] != (heads * hd if heads else shape[1] // hd * hd) or shape[1] == 0 or x.stride(1) != 1:
-        _bad(f"{what} must be [tokens, {heads or 'heads'} * {hd}] with contiguous columns, got {list(shape)}", L.ERR_LENGTH)
+    shape = x.shape
+    if len(shape) == 2:
+        tokens, width = shape
+        step, col = x.stride()
+        n = width // cache.head_dim
+        if n and n * cache.head_dim == width and (n == heads or heads == 0) and col == 1 and x.get_device() == cache._index:
+            return tokens, n, step if tokens > 1 else max(width, step)
     if x.device != cache.device:
         _bad(f"{what} is on {x.device}, the cache on {cache.device}")
-    return shape[0], shape[1] // hd, x.stride(0) if shape[0] > 1 else max(shape[1], x.stride(0))
+    _bad(f"{what} must be [tokens, {heads or 'heads'} * {cache.head_dim}] with contiguous columns, got {list(shape)}", L.ERR_LENGTH)
 
 
-def _small(x: Optional[torch.Tensor], dtype, n: int, device, what: str) -> int:
-    if x is None:
-        return 0
+def _small(x: torch.Tensor, dtype, n: int, device, what: str) -> int:
     if x.dtype != dtype or x.dim() != 1 or x.shape[0] != n or x.device != device or not x.is_contiguous():
         _bad(f"{what} must be {n} contiguous {dtype} values on {device}")
     return x.data_ptr()
@@ -144,22 +147,25 @@ def paged_rope_append(batch: PagedBatch, q: Optional[torch.Tensor], k: torch.Ten
     tokens, _, ks = _rows(k, cache.kv_heads, cache, "paged_rope_append: k")
     v_tokens, _, vs = _rows(v, cache.kv_heads, cache, "paged_rope_append: v")
     q_tokens, heads, qs = (tokens, 0, 0) if q is None else _rows(q, 0, cache, "paged_rope_append: q")
-    _want(v_tokens == tokens == q_tokens, "paged_rope_append: q, k and v differ in tokens", L.ERR_LENGTH)
+    if not v_tokens == tokens == q_tokens:
+        _bad("paged_rope_append: q, k and v differ in tokens", L.ERR_LENGTH)
     x_dtype = _DTYPE.get(k.dtype)
-    _want(x_dtype is not None and v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "paged_rope_append: q, k and v must be f32, bf16 or f16, all the same",
-          L.ERR_NOT_SUPPORTED)
-    _want(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous() and
-          cos.device == sin.device == dev, "paged_rope_append: cos and sin must be contiguous f32 [n_pos, rot_dim / 2] on the cache's device")
-    pos = _small(positions, torch.int32, tokens, dev, "paged_rope_append: positions")
+    if x_dtype is None or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        _bad("paged_rope_append: q, k and v must be f32, bf16 or f16, all the same", L.ERR_NOT_SUPPORTED)
+    table = cos.shape
+    if not (len(table) == 2 and table == sin.shape and cos.dtype is sin.dtype is torch.float32 and cos.is_contiguous() and sin.is_contiguous() and
+            cos.get_device() == sin.get_device() == cache._index):
+        _bad("paged_rope_append: cos and sin must be contiguous f32 [n_pos, rot_dim / 2] on the cache's device")
+    pos = 0 if positions is None else _small(positions, torch.int32, tokens, dev, "paged_rope_append: positions")
     if q is None:
         _want(q_out is None, "paged_rope_append: q_out without q")
     elif q_out is None:
-        q_out = torch.empty(tokens, heads * cache.head_dim, dtype=cache.dtype, device=dev)
+        q_out = cache.k.new_empty((tokens, heads * cache.head_dim))
     else:
         _want(q_out.shape == q.shape and q_out.dtype == cache.dtype and q_out.device == dev and q_out.is_contiguous(),
               "paged_rope_append: q_out must be contiguous, of q's shape and the cache's type")
     _run(cache, L.load().qb200_paged_rope_append, cache._ref, batch._ref, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), x_dtype, qs, ks, vs,
-         tokens, heads, cos.data_ptr(), sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], pos, 0 if q is None else q_out.data_ptr())
+         tokens, heads, cos.data_ptr(), sin.data_ptr(), 2 * table[1], table[0], pos, 0 if q is None else q_out.data_ptr())
     return q_out
 
 
@@ -171,12 +177,12 @@ def _attend(who: str, batch: PagedBatch, q: torch.Tensor, slopes, out, lse):
     if q.dtype != cache.dtype:
         _bad(f"{who}: q is {q.dtype}, the cache {cache.dtype}", L.ERR_NOT_SUPPORTED)
     if out is None:
-        out = torch.empty(q.shape, dtype=cache.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != cache.dtype or out.device != dev or not out.is_contiguous():
         _bad(f"{who}: out must be contiguous, of q's shape and the cache's type")
     if lse is not None and (lse.shape != (tokens, heads) or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous()):
         _bad(f"{who}: lse must be contiguous f32 [{tokens}, {heads}]")
-    return tokens, heads, qs, _small(slopes, torch.float32, heads, dev, who), out, 0 if lse is None else lse.data_ptr()
+    return tokens, heads, qs, 0 if slopes is None else _small(slopes, torch.float32, heads, dev, who + ": slopes"), out, 0 if lse is None else lse.data_ptr()
 
 
 def _scratch(who: str, batch: PagedBatch, scratch: Optional[torch.Tensor], size_of, *shape) -> torch.Tensor:
@@ -187,10 +193,12 @@ def _scratch(who: str, batch: PagedBatch, scratch: Optional[torch.Tensor], size_
     if floats is None:
         if cache._index < 0:
             _bad("the cache is not on a CUDA device", L.ERR_CUDA)
+        if len(batch._floats) >= 1024:
+            batch._floats.clear()
         with torch.cuda.device(cache._index):
             floats = batch._floats[shape] = size_of(cache._ref, batch._ref, *shape)
     if scratch is None:
-        return torch.empty(floats, dtype=torch.float32, device=cache.device)
+        return cache._f32.new_empty(floats)
     if scratch.dtype != torch.float32 or scratch.device != cache.device or not scratch.is_contiguous() or scratch.numel() < floats:
         _bad(f"{who}: scratch must be {floats} contiguous f32 values on {cache.device}", L.ERR_LENGTH)
     return scratch
@@ -206,7 +214,7 @@ def paged_attention(batch: PagedBatch, q: torch.Tensor, scale: Optional[float] =
     f32 receives the log of each row's sum of exp(score).  A row that sees no key gives zeros and -inf."""
     cache = batch.cache
     tokens, heads, qs, sl, out, lp = _attend("paged_attention", batch, q, slopes, out, lse)
-    pl = _small(prefix_lens, torch.int32, batch.size, cache.device, "paged_attention: prefix_lens")
+    pl = 0 if prefix_lens is None else _small(prefix_lens, torch.int32, batch.size, cache.device, "paged_attention: prefix_lens")
     lib = L.load()
     scratch = _scratch("paged_attention", batch, scratch, lib.qb200_paged_attention_scratch_floats, tokens, heads)
     _run(cache, lib.qb200_paged_attention, cache._ref, batch._ref, q.data_ptr(), qs, tokens, heads, cache._scale if scale is None else scale, softcap, sl, pl,
@@ -222,10 +230,12 @@ def shared_prefix_attention(batch: PagedBatch, q: torch.Tensor, prefix_pages: to
     all tokens.  A token's place counts from the prefix's first key."""
     cache = batch.cache
     tokens, heads, qs, sl, out, lp = _attend("shared_prefix_attention", batch, q, slopes, out, lse)
+    if prefix_len <= 0:
+        _bad("shared_prefix_attention: the prefix is empty (call paged_attention)")
     need = -(-prefix_len // cache.page_size)
-    _want(prefix_len > 0, "shared_prefix_attention: the prefix is empty (call paged_attention)")
-    _want(prefix_pages.dim() == 1 and prefix_pages.dtype == torch.int32 and prefix_pages.is_contiguous() and prefix_pages.device == cache.device and
-          prefix_pages.shape[0] >= need, f"shared_prefix_attention: {prefix_len} keys need {need} contiguous int32 page numbers on {cache.device}", L.ERR_LENGTH)
+    if prefix_pages.dim() != 1 or prefix_pages.dtype != torch.int32 or not prefix_pages.is_contiguous() or prefix_pages.get_device() != cache._index or \
+            prefix_pages.shape[0] < need:
+        _bad(f"shared_prefix_attention: {prefix_len} keys need {need} contiguous int32 page numbers on {cache.device}", L.ERR_LENGTH)
     lib = L.load()
     scratch = _scratch("shared_prefix_attention", batch, scratch, lib.qb200_shared_prefix_scratch_floats, prefix_len, tokens, heads)
     _run(cache, lib.qb200_shared_prefix_attention, cache._ref, batch._ref, prefix_pages.data_ptr(), prefix_len, q.data_ptr(), qs, tokens, heads,
