@@ -238,7 +238,8 @@ static qb200_status pg_sms(uint32_t* n) {
 // only the device knows the lengths, both are launched.
 struct PgPlan {
     bool few, many;
-    uint32_t min_rows, grid, splits;
+    uint32_t min_rows, splits;
+    PgRows rows;
     uint64_t floats;  // scratch: the kernels follow one another and share it
 };
 static PgPlan pg_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
@@ -248,8 +249,8 @@ static PgPlan pg_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
     p.few = !p.many || (!a.shared && a.cu_q && a.group <= PG_FEW_ROWS);
     p.min_rows = p.few ? PG_FEW_ROWS + 1 : 1;
     if (p.few) {
-        p.grid = pg_rows_grid(a, sms);
-        p.floats = pg_rows_part_floats(p.grid, hd);
+        p.rows = pg_rows_plan(a, hd, sms);
+        p.floats = p.rows.floats;
     }
     if (p.many) {
         p.splits = pg_prompt_splits(a, sms);
@@ -270,8 +271,8 @@ static qb200_status pg_phase(PgArgs a, int dtype, uint32_t hd, uint32_t sms, flo
     }
     if (p.few) {
         a.meta = reinterpret_cast<int32_t*>(scratch);
-        a.parts = scratch + (uint64_t)p.grid * 8;
-        return pg_rows_launch(a, dtype, hd, p.grid, st);
+        a.parts = scratch + (uint64_t)p.rows.grid * 8;
+        return pg_rows_launch(a, dtype, hd, p.rows, st);
     }
     return QB200_OK;
 }

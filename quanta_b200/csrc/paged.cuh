@@ -207,30 +207,42 @@ __device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_
     pg_store4<T, HD>(a, pg_end(a, token, head, m, l, col == 0), col, v);
 }
 
-// Attention over packed rows (paged_rows.cu): grid of CTAs and floats of partial results it may use.
+// Attention for few rows (paged_rows.cu): how it runs and the floats of partial results that takes.
+struct PgRows {
+    bool units;      // a cluster of 2^c_log CTAs per unit; otherwise equal runs of all tiles, and a second kernel
+    uint32_t c_log, grid;
+    uint64_t floats;
+};
 uint64_t pg_rows_most_tiles(const PgArgs& a);  // below 2^32, or the call is refused
-uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms);
-uint64_t pg_rows_part_floats(uint32_t grid, uint32_t hd);
-qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t grid, cudaStream_t st);
+PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms);
+qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, const PgRows& how, cudaStream_t st);
 // Attention for many rows (paged_prompt.cu): over how many ranges a unit's keys are cut, the floats of partial results
 // that takes, and the launch; min_rows: sequences of fewer packed rows are not its own.
 uint32_t pg_prompt_splits(const PgArgs& a, uint32_t sms);
 uint64_t pg_prompt_part_floats(const PgArgs& a, uint32_t splits, uint32_t hd);
 qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t splits, uint32_t min_rows, cudaStream_t st);
 
+// Launches with programmatic stream serialization (see the kernels' first lines), in clusters of `cluster` CTAs.
 template <typename... KArgs, typename... Args>
-static cudaError_t pg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, uint32_t smem, cudaStream_t st, Args... args) {
+static cudaError_t pg_launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, uint32_t smem, cudaStream_t st, uint32_t cluster, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+static cudaError_t pg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, uint32_t smem, cudaStream_t st, Args... args) {
+    return pg_launch_cluster(kernel, grid, block, smem, st, 1, args...);
 }
 
 }  // namespace qb

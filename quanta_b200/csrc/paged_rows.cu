@@ -66,6 +66,12 @@ __device__ __forceinline__ uint32_t pr_weight(const PgArgs& a, const PgSeq& s) {
     return rows == 0 || rows > PG_FEW_ROWS ? 0 : a.kv_heads * pr_tiles(s);
 }
 
+// Tiles of a CTA up to which units are given to clusters (where the CTAs leave SMs idle, and where they do not).  Clusters
+// need no search and no second launch, equal runs balance long ragged batches and cut single long sequences finer.  Us
+// by clusters / by runs, K/V heads x sequences x keys: 8 x 1 x 1024 5.1 / 7.1, 8 x 1 x 4096 8.8 / 10.6, 8 x 1 x 16384 25 / 19;
+// 32 x 16 x 1024 42 / 46, 8 x 64 x 2048 80 / 84 (lengths up to 2048: 51 / 54), 8 x 64 x 8192 301 / 313 (up to 8192: 190 / 172).
+constexpr uint32_t PR_SHORT = 8, PR_LONG = 32;
+
 // Sequences whose lengths the CTA keeps in shared memory: the first ones of the call.
 constexpr uint32_t PR_KEPT = PR_WARPS * 32;
 
@@ -154,6 +160,197 @@ __device__ __forceinline__ void pr_advance(const PgArgs& a, const PgSeq* kept, P
     p.tiles = pr_tiles(p.s);
 }
 
+// What a warp holds of a unit: a thread has rows lane / 4 and lane / 4 + 8.
+template <uint32_t HD> struct PrState {
+    float m[2], l[2], o[HD / 8][4];
+    uint32_t lim[2];  // keys the rows see, and the bias they get
+    float slope[2];
+    int32_t pos[2];
+};
+template <uint32_t HD, bool SCORED>
+__device__ __forceinline__ void pr_begin(const PgArgs& a, const PgSeq& sq, uint32_t kvh, PrState<HD>& u) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2; i++) {
+        const uint32_t r = ((threadIdx.x & 31) >> 2) + 8 * i;
+        u.m[i] = -INFINITY;
+        u.l[i] = 0.0f;
+        u.lim[i] = 0;
+        u.slope[i] = 0.0f;
+        u.pos[i] = 0;
+        if (r < sq.q_len * a.group) {
+            u.lim[i] = pg_limit(sq, r / a.group);
+            if (SCORED && a.slopes) {
+                u.slope[i] = a.slopes[kvh * a.group + r % a.group] * PG_LOG2E;
+                u.pos[i] = pg_position(a, sq, r / a.group);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < HD / 8; k++) u.o[k][0] = u.o[k][1] = u.o[k][2] = u.o[k][3] = 0.0f;
+}
+// A 16-byte chunk of the unit's 16 rows of Q (zeros past the last row).
+template <uint32_t HD>
+__device__ __forceinline__ uint4 pr_load_q(const PgArgs& a, const PgSeq& sq, uint32_t kvh, uint32_t id) {
+    const uint32_t r = id / (HD / 8), c = id % (HD / 8);
+    if (r >= sq.q_len * a.group) return make_uint4(0, 0, 0, 0);
+    return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + r / a.group) * a.q_stride +
+                                           (uint64_t)(kvh * a.group + r % a.group) * HD + c * 8);
+}
+template <uint32_t HD> __device__ __forceinline__ uint32_t pr_q_place(uint32_t id) {
+    const uint32_t r = id / (HD / 8), c = id % (HD / 8);
+    return r * (HD * 2) + ((c ^ (r & 7)) << 4);
+}
+template <uint32_t HD> __device__ __forceinline__ void pr_q_fragments(uint32_t q_s, uint32_t (&qf)[HD / 16][4]) {
+    const uint32_t lane = threadIdx.x & 31, r = (((lane >> 3) & 1) << 3) | (lane & 7), sub = lane >> 4;
+#pragma unroll
+    for (uint32_t ks = 0; ks < HD / 16; ks++) pr_ldsm(q_s + r * (HD * 2) + (((ks * 2 + sub) ^ (r & 7)) << 4), qf[ks]);
+}
+// 16 keys of a page and head to a stage (K, then V; 16-byte chunk c of a row at c ^ (row & 7)): `valid` of them, the
+// others are zeros, whatever the page holds there, and so are all keys of a page that is not in the pool.
+template <uint32_t HD>
+__device__ __forceinline__ void pr_copy_keys(const PgArgs& a, uint32_t dst, int32_t page, uint32_t kvh, uint32_t key, uint32_t valid, uint64_t once) {
+    constexpr uint32_t CH = HD / 8, ROW = HD * 2;
+    if (valid && (uint32_t)page >= a.n_pages) {
+        pg_report(a.status, QB200_ERR_INVALID_PARAM);
+        valid = 0;
+    }
+    const uint64_t base = valid ? (((uint64_t)(uint32_t)page * a.kv_heads + kvh) << a.ps_log) + (key & ((1u << a.ps_log) - 1)) : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < PR_KEYS * CH / 32; i++) {
+        const uint32_t id = i * 32 + (threadIdx.x & 31), row = id / CH, c = id % CH, bytes = row < valid ? 16u : 0u;
+        const uint64_t src = (base + (bytes ? row : 0)) * HD + c * 8;
+        const uint32_t d = dst + row * ROW + ((c ^ (row & 7)) << 4);
+        pr_copy16(d, a.k + src, bytes, once);
+        pr_copy16(d + PR_KEYS * ROW, a.v + src, bytes, once);
+    }
+}
+// One tile: the warp's 16 keys, from `first` on, in the stage at ks_s.
+template <typename T, uint32_t HD, bool SCORED>
+__device__ __forceinline__ void pr_step(const PgArgs& a, uint32_t ks_s, uint32_t first, const uint32_t (&qf)[HD / 16][4], PrState<HD>& u) {
+    using S = PrShape<HD>;
+    constexpr uint32_t KS = HD / 16, NP = HD / 16;
+    const uint32_t lane = threadIdx.x & 31, part4 = lane & 3, vs_s = ks_s + PR_KEYS * S::ROW;
+    float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    {
+        const uint32_t key = ((lane >> 4) << 3) | (lane & 7), sub = (lane >> 3) & 1;
+#pragma unroll
+        for (uint32_t ks = 0; ks < KS; ks++) {
+            uint32_t kf[4];
+            pr_ldsm(ks_s + key * S::ROW + (((ks * 2 + sub) ^ (key & 7)) << 4), kf);
+            pr_mma(s[0], qf[ks], kf[0], kf[1], T());
+            pr_mma(s[1], qf[ks], kf[2], kf[3], T());
+        }
+    }
+    const uint32_t key0 = first + part4 * 2;
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (uint32_t k = 0; k < 2; k++)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t r = i >> 1, key = key0 + k * 8 + (i & 1);
+            float x = s[k][i] * a.score_mul;
+            if (SCORED) {
+                if (a.cap_mul != 0.0f) x = pg_cap(x, a.cap_mul);
+                x = fmaf(-u.slope[r], fabsf((float)(u.pos[r] - (int32_t)key)), x);
+            }
+            x = key < u.lim[r] ? x : -INFINITY;
+            s[k][i] = x;
+            mx[r] = fmaxf(mx[r], x);
+        }
+    float f[2], ms[2];
+#pragma unroll
+    for (uint32_t r = 0; r < 2; r++) {
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xFFFFFFFFu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xFFFFFFFFu, mx[r], 2));
+        const float mn = fmaxf(u.m[r], mx[r]);
+        ms[r] = mn == -INFINITY ? 0.0f : mn;
+        f[r] = pg_exp2(u.m[r] - ms[r]);
+        u.m[r] = mn;
+        u.l[r] *= f[r];
+    }
+    if (__any_sync(0xFFFFFFFFu, f[0] != 1.0f || f[1] != 1.0f)) {
+#pragma unroll
+        for (uint32_t k = 0; k < 2 * NP; k++) {
+            u.o[k][0] *= f[0];
+            u.o[k][1] *= f[0];
+            u.o[k][2] *= f[1];
+            u.o[k][3] *= f[1];
+        }
+    }
+    uint32_t pf[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 2; k++) {
+        float p[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            p[i] = pg_exp2(s[k][i] - ms[i >> 1]);
+            u.l[i >> 1] += p[i];
+        }
+        pf[k * 2] = PgType<T>::pack(p[0], p[1]);
+        pf[k * 2 + 1] = PgType<T>::pack(p[2], p[3]);
+    }
+    {
+        const uint32_t key = (((lane >> 3) & 1) << 3) | (lane & 7), sub = lane >> 4;
+#pragma unroll
+        for (uint32_t k = 0; k < NP; k++) {
+            uint32_t vf[4];
+            pr_ldsm_t(vs_s + key * S::ROW + (((k * 2 + sub) ^ (key & 7)) << 4), vf);
+            pr_mma(u.o[2 * k], pf, vf[0], vf[1], T());
+            pr_mma(u.o[2 * k + 1], pf, vf[2], vf[3], T());
+        }
+    }
+}
+// The sums of a thread's two rows over the four threads that share them, and the row's (m, l) to ml [2][16].
+template <uint32_t HD> __device__ __forceinline__ void pr_end(PrState<HD>& u, float* ml) {
+    const uint32_t lane = threadIdx.x & 31, quad = lane >> 2;
+#pragma unroll
+    for (uint32_t r = 0; r < 2; r++) {
+        u.l[r] += __shfl_xor_sync(0xFFFFFFFFu, u.l[r], 1);
+        u.l[r] += __shfl_xor_sync(0xFFFFFFFFu, u.l[r], 2);
+    }
+    if ((lane & 3) == 0) {
+        ml[quad] = u.m[0];
+        ml[quad + 8] = u.m[1];
+        ml[PR_ROWS + quad] = u.l[0];
+        ml[PR_ROWS + quad + 8] = u.l[1];
+    }
+}
+// Rows [p0, p0 + PASS) of the warp's accumulator to the join area.
+template <uint32_t HD> __device__ __forceinline__ void pr_put_rows(const PrState<HD>& u, float* j_acc, uint32_t p0) {
+    using S = PrShape<HD>;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (uint32_t i = 0; i < 2; i++) {
+        const uint32_t r = (lane >> 2) + 8 * i - p0;
+        if (r < S::PASS) {
+            float* to = j_acc + (warp * S::PASS + r) * S::ACC + (lane & 3) * 2;
+#pragma unroll
+            for (uint32_t k = 0; k < HD / 8; k++) *reinterpret_cast<float2*>(to + k * 8) = make_float2(u.o[k][2 * i], u.o[k][2 * i + 1]);
+        }
+    }
+}
+// Four columns of row r over the CTA's warps.
+template <uint32_t HD>
+__device__ __forceinline__ float4 pr_join_warps(const float* j_acc, const float* j_ml, uint32_t r, uint32_t p0, uint32_t col, float& M, float& L) {
+    using S = PrShape<HD>;
+    M = -INFINITY;
+#pragma unroll
+    for (uint32_t w = 0; w < PR_WARPS; w++) M = fmaxf(M, j_ml[w * 2 * PR_ROWS + r]);
+    L = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t w = 0; w < PR_WARPS; w++) {
+        const float g = pg_weight(j_ml[w * 2 * PR_ROWS + r], M);
+        const float4 e = *reinterpret_cast<const float4*>(j_acc + (w * S::PASS + r - p0) * S::ACC + col);
+        L = fmaf(j_ml[w * 2 * PR_ROWS + PR_ROWS + r], g, L);
+        v.x = fmaf(e.x, g, v.x);
+        v.y = fmaf(e.y, g, v.y);
+        v.z = fmaf(e.z, g, v.z);
+        v.w = fmaf(e.w, g, v.w);
+    }
+    return v;
+}
+
 template <typename T, uint32_t HD, bool SCORED>
 __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_constant__ PgArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -161,8 +358,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
     using S = PrShape<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PgSeq kept[PR_KEPT];
-    constexpr uint32_t KS = HD / 16, NP = HD / 16, CH = HD / 8;  // k-steps of S, pairs of column tiles of O, 16-byte chunks of a row
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane >> 2, part4 = lane & 3;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5;
     int32_t* meta = a.meta + blockIdx.x * 8;
     if (tid == 0) meta[0] = -1;
     PrRun run;
@@ -180,9 +376,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
     here.left = run.run1 - run.run0;
     ahead = here;
 
-    // ---- the ring: the warp's 16 keys of one tile a stage (16-byte chunk c of a row at c ^ (row & 7)).  Keys behind the
-    // sequence's last one are zeros, whatever the page holds there, and so are all keys of a page that is not in the pool.
-    // The next tile's page number is read a step before it is needed.
+    // ---- the ring: the warp's 16 keys of one tile a stage.  The next tile's page number is read a step before it is needed. ----
     const uint64_t once = pr_once();
     int32_t n_page = 0;
     uint32_t n_kvh = 0, n_key = 0, n_valid = 0;
@@ -198,37 +392,18 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
     };
     auto fetch = [&](uint32_t st) {
         if (n_there) {
-            if (n_valid && (uint32_t)n_page >= a.n_pages) {
-                pg_report(a.status, QB200_ERR_INVALID_PARAM);
-                n_valid = 0;
-            }
-            const uint64_t base = n_valid ? (((uint64_t)(uint32_t)n_page * a.kv_heads + n_kvh) << a.ps_log) + (n_key & ((1u << a.ps_log) - 1)) : 0;
-            const uint32_t dst = ring_s + st * S::STAGE;
-#pragma unroll
-            for (uint32_t i = 0; i < PR_KEYS * CH / 32; i++) {
-                const uint32_t id = i * 32 + lane, row = id / CH, c = id % CH, bytes = row < n_valid ? 16u : 0u;
-                const uint64_t src = (base + (bytes ? row : 0)) * HD + c * 8;
-                const uint32_t d = dst + row * S::ROW + ((c ^ (row & 7)) << 4);
-                pr_copy16(d, a.k + src, bytes, once);
-                pr_copy16(d + PR_KEYS * S::ROW, a.v + src, bytes, once);
-            }
+            pr_copy_keys<HD>(a, ring_s + st * S::STAGE, n_page, n_kvh, n_key, n_valid, once);
             look();
         }
         pr_commit();
     };
 
     // ---- Q of a unit: loaded while the unit before it is joined, then through shared memory into fragments ----
-    constexpr uint32_t QN = PR_ROWS * CH / 128;  // 16-byte chunks a thread brings
+    constexpr uint32_t QN = PR_ROWS * (HD / 8) / 128;  // 16-byte chunks a thread brings
     uint4 q_in[QN];
     auto bring_q = [&](const PrAt& p) {
 #pragma unroll
-        for (uint32_t i = 0; i < QN; i++) {
-            const uint32_t id = i * 128 + tid, r = id / CH, c = id % CH;
-            q_in[i] = make_uint4(0, 0, 0, 0);
-            if (r < p.s.q_len * a.group)
-                q_in[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(p.s.q0 + r / a.group) * a.q_stride +
-                                                          (uint64_t)(p.kvh * a.group + r % a.group) * HD + c * 8);
-        }
+        for (uint32_t i = 0; i < QN; i++) q_in[i] = pr_load_q<HD>(a, p.s, p.kvh, i * 128 + tid);
     };
 
     bring_q(here);
@@ -239,115 +414,21 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
     while (true) {
         // ---- a unit ----
 #pragma unroll
-        for (uint32_t i = 0; i < QN; i++) {
-            const uint32_t id = i * 128 + tid, r = id / CH, c = id % CH;
-            *reinterpret_cast<uint4*>(smem + S::Q + r * S::ROW + ((c ^ (r & 7)) << 4)) = q_in[i];
-        }
+        for (uint32_t i = 0; i < QN; i++) *reinterpret_cast<uint4*>(smem + S::Q + pr_q_place<HD>(i * 128 + tid)) = q_in[i];
         __syncthreads();
-        uint32_t qf[KS][4];
-        {
-            const uint32_t r = (((lane >> 3) & 1) << 3) | (lane & 7), sub = lane >> 4;
-#pragma unroll
-            for (uint32_t ks = 0; ks < KS; ks++) pr_ldsm(q_s + r * S::ROW + (((ks * 2 + sub) ^ (r & 7)) << 4), qf[ks]);
-        }
+        uint32_t qf[HD / 16][4];
+        pr_q_fragments<HD>(q_s, qf);
         const PgSeq sq = here.s;
         const uint32_t kvh = here.kvh, rows = sq.q_len * a.group, t0 = here.t, n = min(here.tiles - t0, here.left);
         const bool whole = n == here.tiles;
-        // this thread's two rows: what they see, and the bias they get
-        uint32_t lim[2];
-        float slope[2];
-        int32_t pos[2];
-#pragma unroll
-        for (uint32_t i = 0; i < 2; i++) {
-            const uint32_t r = quad + 8 * i;
-            lim[i] = 0;
-            slope[i] = 0.0f;
-            pos[i] = 0;
-            if (r < rows) {
-                lim[i] = pg_limit(sq, r / a.group);
-                if (SCORED && a.slopes) {
-                    slope[i] = a.slopes[kvh * a.group + r % a.group] * PG_LOG2E;
-                    pos[i] = pg_position(a, sq, r / a.group);
-                }
-            }
-        }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2 * NP][4];
-#pragma unroll
-        for (uint32_t k = 0; k < 2 * NP; k++) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.0f;
+        PrState<HD> u;
+        pr_begin<HD, SCORED>(a, sq, kvh, u);
 
         for (uint32_t t = t0; t < t0 + n; t++) {
             pr_wait<S::STAGES - 2>();
             __syncwarp();
-            const uint32_t ks_s = ring_s + st * S::STAGE, vs_s = ks_s + PR_KEYS * S::ROW;
-            float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-            {
-                const uint32_t key = ((lane >> 4) << 3) | (lane & 7), sub = (lane >> 3) & 1;
-#pragma unroll
-                for (uint32_t ks = 0; ks < KS; ks++) {
-                    uint32_t kf[4];
-                    pr_ldsm(ks_s + key * S::ROW + (((ks * 2 + sub) ^ (key & 7)) << 4), kf);
-                    pr_mma(s[0], qf[ks], kf[0], kf[1], T());
-                    pr_mma(s[1], qf[ks], kf[2], kf[3], T());
-                }
-            }
-            const uint32_t key0 = t * PR_TILE + warp * PR_KEYS + part4 * 2;
-            float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (uint32_t k = 0; k < 2; k++)
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) {
-                    const uint32_t r = i >> 1, key = key0 + k * 8 + (i & 1);
-                    float x = s[k][i] * a.score_mul;
-                    if (SCORED) {
-                        if (a.cap_mul != 0.0f) x = pg_cap(x, a.cap_mul);
-                        x = fmaf(-slope[r], fabsf((float)(pos[r] - (int32_t)key)), x);
-                    }
-                    x = key < lim[r] ? x : -INFINITY;
-                    s[k][i] = x;
-                    mx[r] = fmaxf(mx[r], x);
-                }
-            float f[2], ms[2];
-#pragma unroll
-            for (uint32_t r = 0; r < 2; r++) {
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xFFFFFFFFu, mx[r], 1));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xFFFFFFFFu, mx[r], 2));
-                const float mn = fmaxf(m[r], mx[r]);
-                ms[r] = mn == -INFINITY ? 0.0f : mn;
-                f[r] = pg_exp2(m[r] - ms[r]);
-                m[r] = mn;
-                l[r] *= f[r];
-            }
-            if (__any_sync(0xFFFFFFFFu, f[0] != 1.0f || f[1] != 1.0f)) {
-#pragma unroll
-                for (uint32_t k = 0; k < 2 * NP; k++) {
-                    o[k][0] *= f[0];
-                    o[k][1] *= f[0];
-                    o[k][2] *= f[1];
-                    o[k][3] *= f[1];
-                }
-            }
-            uint32_t pf[4];
-#pragma unroll
-            for (uint32_t k = 0; k < 2; k++) {
-                float p[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) {
-                    p[i] = pg_exp2(s[k][i] - ms[i >> 1]);
-                    l[i >> 1] += p[i];
-                }
-                pf[k * 2] = PgType<T>::pack(p[0], p[1]);
-                pf[k * 2 + 1] = PgType<T>::pack(p[2], p[3]);
-            }
-            {
-                const uint32_t key = (((lane >> 3) & 1) << 3) | (lane & 7), sub = lane >> 4;
-#pragma unroll
-                for (uint32_t k = 0; k < NP; k++) {
-                    uint32_t vf[4];
-                    pr_ldsm_t(vs_s + key * S::ROW + (((k * 2 + sub) ^ (key & 7)) << 4), vf);
-                    pr_mma(o[2 * k], pf, vf[0], vf[1], T());
-                    pr_mma(o[2 * k + 1], pf, vf[2], vf[3], T());
-                }
-            }
+            const uint32_t ks_s = ring_s + st * S::STAGE;
+            pr_step<T, HD, SCORED>(a, ks_s, t * PR_TILE + warp * PR_KEYS, qf, u);
             __syncwarp();  // every lane is done with the stage that the next fetch overwrites: the one before this
             fetch(st == 0 ? S::STAGES - 1 : st - 1);
             if (++st == S::STAGES) st = 0;
@@ -358,18 +439,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
         pr_advance(a, kept, here, n);
         const bool more = here.left != 0;
         if (more) bring_q(here);
-#pragma unroll
-        for (uint32_t r = 0; r < 2; r++) {
-            l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
-        }
-        if (part4 == 0) {
-            float* ml = j_ml + warp * 2 * PR_ROWS;
-            ml[quad] = m[0];
-            ml[quad + 8] = m[1];
-            ml[PR_ROWS + quad] = l[0];
-            ml[PR_ROWS + quad + 8] = l[1];
-        }
+        pr_end<HD>(u, j_ml + warp * 2 * PR_ROWS);
         float* part = a.parts + ((uint64_t)blockIdx.x * 2 + slot) * S::PART;
         if (!whole && t0 == 0 && tid == 0) {  // a unit that starts here and goes on: what the second kernel joins
             const uint32_t x = first_tile + (whole ? n : pr_tiles(sq)) - 1, cut = run.extra * (run.base + 1);
@@ -382,34 +452,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
         constexpr uint32_t PER = HD / 4;  // threads of a row
         for (uint32_t p0 = 0; p0 < rows; p0 += S::PASS) {
             if (p0) __syncthreads();  // the rows before have been read
-#pragma unroll
-            for (uint32_t i = 0; i < 2; i++) {
-                const uint32_t r = quad + 8 * i - p0;
-                if (r < S::PASS) {
-                    float* to = j_acc + (warp * S::PASS + r) * S::ACC + part4 * 2;
-#pragma unroll
-                    for (uint32_t k = 0; k < 2 * NP; k++) *reinterpret_cast<float2*>(to + k * 8) = make_float2(o[k][2 * i], o[k][2 * i + 1]);
-                }
-            }
+            pr_put_rows<HD>(u, j_acc, p0);
             __syncthreads();
 #pragma unroll 1
             for (uint32_t r = p0 + tid / PER; r < min(rows, p0 + S::PASS); r += PR_WARPS * 32 / PER) {
                 const uint32_t col = (tid % PER) * 4;
-                float M = -INFINITY;
-#pragma unroll
-                for (uint32_t w = 0; w < PR_WARPS; w++) M = fmaxf(M, j_ml[w * 2 * PR_ROWS + r]);
-                float L = 0.0f;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (uint32_t w = 0; w < PR_WARPS; w++) {
-                    const float g = pg_weight(j_ml[w * 2 * PR_ROWS + r], M);
-                    const float4 e = *reinterpret_cast<const float4*>(j_acc + (w * S::PASS + r - p0) * S::ACC + col);
-                    L = fmaf(j_ml[w * 2 * PR_ROWS + PR_ROWS + r], g, L);
-                    v.x = fmaf(e.x, g, v.x);
-                    v.y = fmaf(e.y, g, v.y);
-                    v.z = fmaf(e.z, g, v.z);
-                    v.w = fmaf(e.w, g, v.w);
-                }
+                float M, L;
+                const float4 v = pr_join_warps<HD>(j_acc, j_ml, r, p0, col, M, L);
                 if (whole) {
                     pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
                 } else {
@@ -426,6 +475,125 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
         __syncthreads();  // the join area is free again
     }
     pr_wait<0>();
+}
+
+// The same for tables of moderate length, in one launch and without a search: a unit has a cluster of 2^c_log CTAs, each
+// takes an equal range of its tiles, and their states meet in the cluster's shared memory.
+template <typename T, uint32_t HD, bool SCORED>
+__global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_constant__ PgArgs a, uint32_t c_log) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    using S = PrShape<HD>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5;
+    const uint32_t rank = blockIdx.x & ((1u << c_log) - 1), unit = blockIdx.x >> c_log, b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
+    const PgSeq sq = pg_seq(a, b);
+    const uint32_t rows = sq.q_len * a.group;
+    if (rows == 0 || rows > PG_FEW_ROWS) return;  // the whole cluster alike
+    const uint32_t ring_s = pr_smem(smem + warp * S::WARP), q_s = pr_smem(smem + S::Q);
+    float* j_acc = reinterpret_cast<float*>(smem + S::JOIN);
+    float* j_ml = reinterpret_cast<float*>(smem + S::ML);
+    const uint64_t once = pr_once();
+    const uint32_t tiles = pr_tiles(sq), t0 = tiles * rank >> c_log, t1 = tiles * (rank + 1) >> c_log;
+    const int32_t* table = a.table + (a.shared ? 0 : (uint64_t)b * a.table_stride);
+    uint32_t ahead = t0;  // the next tile to fetch, and its page
+    int32_t page = 0;
+    auto look = [&]() {
+        const uint32_t key = ahead * PR_TILE + warp * PR_KEYS;
+        if (ahead < t1 && key < sq.kv) page = table[key >> a.ps_log];
+    };
+    auto fetch = [&](uint32_t st) {
+        if (ahead < t1) {
+            const uint32_t key = ahead * PR_TILE + warp * PR_KEYS;
+            pr_copy_keys<HD>(a, ring_s + st * S::STAGE, page, kvh, key, key < sq.kv ? min(sq.kv - key, PR_KEYS) : 0, once);
+            ahead++;
+            look();
+        }
+        pr_commit();
+    };
+    constexpr uint32_t QN = PR_ROWS * (HD / 8) / 128;
+    uint4 q_in[QN];
+#pragma unroll
+    for (uint32_t i = 0; i < QN; i++) q_in[i] = pr_load_q<HD>(a, sq, kvh, i * 128 + tid);
+    look();
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < S::STAGES; i++) fetch(i);
+#pragma unroll
+    for (uint32_t i = 0; i < QN; i++) *reinterpret_cast<uint4*>(smem + S::Q + pr_q_place<HD>(i * 128 + tid)) = q_in[i];
+    __syncthreads();
+    uint32_t qf[HD / 16][4];
+    pr_q_fragments<HD>(q_s, qf);
+    PrState<HD> u;
+    pr_begin<HD, SCORED>(a, sq, kvh, u);
+    uint32_t st = 0;
+    for (uint32_t t = t0; t < t1; t++) {
+        pr_wait<S::STAGES - 2>();
+        __syncwarp();
+        pr_step<T, HD, SCORED>(a, ring_s + st * S::STAGE, t * PR_TILE + warp * PR_KEYS, qf, u);
+        __syncwarp();
+        fetch(st == 0 ? S::STAGES - 1 : st - 1);
+        if (++st == S::STAGES) st = 0;
+    }
+    pr_wait<0>();
+    pr_end<HD>(u, j_ml + warp * 2 * PR_ROWS);
+    // the CTA's state of its rows, in the ring's place (m, l and HD columns a row), then the cluster's
+    constexpr uint32_t PER = HD / 4, ROW = HD + 4;
+    float* mine = reinterpret_cast<float*>(smem);
+    for (uint32_t p0 = 0; p0 < rows; p0 += S::PASS) {
+        if (p0) __syncthreads();  // the rows before have been read
+        pr_put_rows<HD>(u, j_acc, p0);
+        __syncthreads();          // (the first one: no warp reads its ring any more)
+#pragma unroll 1
+        for (uint32_t r = p0 + tid / PER; r < min(rows, p0 + S::PASS); r += PR_WARPS * 32 / PER) {
+            const uint32_t col = (tid % PER) * 4;
+            float M, L;
+            const float4 v = pr_join_warps<HD>(j_acc, j_ml, r, p0, col, M, L);
+            if (c_log == 0) {
+                pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
+                continue;
+            }
+            *reinterpret_cast<float4*>(mine + r * ROW + 4 + col) = v;
+            if (col == 0) *reinterpret_cast<float2*>(mine + r * ROW) = make_float2(M, L);
+        }
+    }
+    if (c_log == 0) return;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const uint32_t peers = 1u << c_log;
+#pragma unroll 1
+    for (uint32_t r = rank + (tid / PER << c_log); r < rows; r += (PR_WARPS * 32 / PER) << c_log) {
+        const uint32_t col = (tid % PER) * 4, at = pr_smem(mine + r * ROW);
+        float m[8], l[8];
+        float4 e[8];
+        float M = -INFINITY, L = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (uint32_t p = 0; p < 8; p++) {
+            m[p] = -INFINITY;
+            l[p] = 0.0f;
+            e[p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (p < peers) {
+                uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(p));
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[p]), "=f"(l[p]) : "r"(there) : "memory");
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e[p].x), "=f"(e[p].y), "=f"(e[p].z), "=f"(e[p].w) : "r"(there + 16 + col * 4) : "memory");
+            }
+        }
+#pragma unroll
+        for (uint32_t p = 0; p < 8; p++) M = fmaxf(M, m[p]);
+#pragma unroll
+        for (uint32_t p = 0; p < 8; p++) {
+            const float g = pg_weight(m[p], M);
+            L = fmaf(l[p], g, L);
+            v.x = fmaf(e[p].x, g, v.x);
+            v.y = fmaf(e[p].y, g, v.y);
+            v.z = fmaf(e[p].z, g, v.z);
+            v.w = fmaf(e[p].w, g, v.w);
+        }
+        pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // no CTA leaves while its state is read
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Joins the partial results of the unit that starts in CTA blockIdx.x's run and ends in a later one's.  A block takes
@@ -519,21 +687,38 @@ uint64_t pg_rows_most_tiles(const PgArgs& a) {
     return (a.shared ? 1 : (uint64_t)a.batch) * a.kv_heads * div_ceil(keys, PR_TILE);
 }
 
-uint32_t pg_rows_grid(const PgArgs& a, uint32_t sms) {
-    const uint64_t most = pg_rows_most_tiles(a);  // two CTAs per SM, fewer where the call cannot have as many tiles
-    return (uint32_t)(most < 2 * sms ? most : 2 * sms);
+PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
+    PgRows how = {};
+    const uint64_t most = pg_rows_most_tiles(a), units = (a.shared ? 1 : (uint64_t)a.batch) * a.kv_heads, tiles = most / units;
+    // A cluster per unit, of up to 8 CTAs while all of them fit the SMs at once, where a CTA then has at most PR_SHORT
+    // tiles, or at most PR_LONG and there are as many CTAs as SMs; equal runs otherwise.
+    uint32_t c_log = 0;
+    while (c_log < 3 && (units << (c_log + 1)) <= 2 * sms && (2u << c_log) <= tiles) c_log++;
+    if (units <= 0x7FFFFFFFull >> c_log && (tiles <= (uint64_t)PR_SHORT << c_log || (tiles <= (uint64_t)PR_LONG << c_log && units << c_log >= sms))) {
+        how.units = true;
+        how.c_log = c_log;
+        how.grid = (uint32_t)(units << c_log);
+        return how;
+    }
+    how.grid = (uint32_t)(most < 2 * sms ? most : 2 * sms);  // two CTAs per SM, fewer where the call cannot have as many tiles
+    how.floats = (uint64_t)how.grid * 2 * PR_ROWS * (hd + 2) + (uint64_t)how.grid * 8;
+    return how;
 }
 
-uint64_t pg_rows_part_floats(uint32_t grid, uint32_t hd) { return (uint64_t)grid * 2 * PR_ROWS * (hd + 2) + (uint64_t)grid * 8; }
-
 template <typename T, uint32_t HD, bool SCORED>
-static qb200_status launch_rows(const PgArgs& a, uint32_t grid, cudaStream_t st) {
+static qb200_status launch_rows(const PgArgs& a, const PgRows& how, cudaStream_t st) {
     static bool attr_set[64] = {};
     int dev = 0;
     QB_CUDA_TRY(cudaGetDevice(&dev));
     if (!attr_set[dev & 63]) {
         QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_rows<T, HD, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrShape<HD>::SMEM));
+        QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_units<T, HD, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrShape<HD>::SMEM));
         attr_set[dev & 63] = true;
+    }
+    const uint32_t grid = how.grid;
+    if (how.units) {
+        QB_CUDA_TRY(pg_launch_cluster(k_paged_units<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, 1u << how.c_log, a, how.c_log));
+        return QB200_OK;
     }
     QB_CUDA_TRY(pg_launch(k_paged_rows<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, a));
     const uint64_t rows = a.cu_q || a.shared ? (uint64_t)a.tokens * a.group : a.group;
@@ -541,14 +726,14 @@ static qb200_status launch_rows(const PgArgs& a, uint32_t grid, cudaStream_t st)
     return QB200_OK;
 }
 
-qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t grid, cudaStream_t st) {
+qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, const PgRows& how, cudaStream_t st) {
     const bool scored = a.cap_mul != 0.0f || a.slopes;
     if (dtype == QB200_BF16) {
-        if (hd == 128) return scored ? launch_rows<__nv_bfloat16, 128, true>(a, grid, st) : launch_rows<__nv_bfloat16, 128, false>(a, grid, st);
-        return scored ? launch_rows<__nv_bfloat16, 64, true>(a, grid, st) : launch_rows<__nv_bfloat16, 64, false>(a, grid, st);
+        if (hd == 128) return scored ? launch_rows<__nv_bfloat16, 128, true>(a, how, st) : launch_rows<__nv_bfloat16, 128, false>(a, how, st);
+        return scored ? launch_rows<__nv_bfloat16, 64, true>(a, how, st) : launch_rows<__nv_bfloat16, 64, false>(a, how, st);
     }
-    if (hd == 128) return scored ? launch_rows<__half, 128, true>(a, grid, st) : launch_rows<__half, 128, false>(a, grid, st);
-    return scored ? launch_rows<__half, 64, true>(a, grid, st) : launch_rows<__half, 64, false>(a, grid, st);
+    if (hd == 128) return scored ? launch_rows<__half, 128, true>(a, how, st) : launch_rows<__half, 128, false>(a, how, st);
+    return scored ? launch_rows<__half, 64, true>(a, how, st) : launch_rows<__half, 64, false>(a, how, st);
 }
 
 }  // namespace qb
