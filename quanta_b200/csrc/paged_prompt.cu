@@ -3,7 +3,7 @@
 // dim 128: 4096 multiply-adds and 16 exponentials a cycle and SM).
 //
 // A unit is 256 packed rows of a sequence and one K/V head, over one of `splits` ranges of its keys; one CTA each, the
-// longest first.  The rows are two tiles of 128 whose steps alternate on the tensor pipe, so that one tile's products
+// longest first (12 prompts of mixed lengths: 312 us with the sequences in the order of the batch, 262 like this, 52 of them other kernels).  The rows are two tiles of 128 whose steps alternate on the tensor pipe, so that one tile's products
 // run under the other's softmax.  Per step of 128 keys and tile: S = Q K^T (tcgen05.mma, both operands in shared
 // memory, accumulator in TMEM), a warpgroup turns S into P (a thread owns a row, so the row's maximum and sum need no
 // exchange), P goes back to TMEM over S in the cache's type, and O += P V takes it from there.  The running maximum a
@@ -145,8 +145,9 @@ __device__ __forceinline__ void pp_mul2(float& x0, float& x1, uint64_t m2) {
     asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tmul.rn.f32x2 t, t, %2;\n\tmov.b64 {%0, %1}, t;\n\t}" : "+f"(x0), "+f"(x1) : "l"(m2));
 }
 // tanh of a pair with |x| <= 1/2: x (1 + u P(u)), u = x^2, P the cubic that is best there (absolute error 4.3e-9, fitted
-// by reweighted least squares), on the multiply-add pipe: seven instructions a pair, where the exponential and the
-// reciprocal of the general form would triple the load of the pipe that already bounds the softmax.
+// by reweighted least squares), on the multiply-add pipe: six instructions a pair, where the exponential and the
+// reciprocal of the general form would triple the load of the pipe that already bounds the softmax.  (The caller scales x:
+// with coefficients multiplied by b^9, b^7, b^5, b^3 and b it is tanh(b x) for |b x| <= 1/2.)
 __device__ __forceinline__ void pp_tanh2(float& x0, float& x1, uint64_t c3, uint64_t c2, uint64_t c1, uint64_t c0, uint64_t one) {
     asm("{\n\t.reg .b64 x, u, p;\n\t"
         "mov.b64 x, {%0, %1};\n\t"
@@ -223,38 +224,66 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pp_before();  // (the barriers of the scan publish all this)
-    // ---- which unit: blocks of all sequences, each sequence's last (longest) block first ----
-    __shared__ uint32_t s_seq, s_before, s_sum[PP_THREADS / 32];
+    // ---- which unit: the sequence with the most keys first, in it the last (longest) block first, so that the CTAs that
+    // start last have the least to do; batches of more sequences than threads go in their own order ----
+    __shared__ uint32_t s_seq, s_before;
+    uint64_t* s_kv = reinterpret_cast<uint64_t*>(sQ);  // keys and blocks of the sequences; in the second form block counts of the warps
     __shared__ PgSeq s_found;
     const uint32_t seqs = a.shared ? 1 : a.batch, want = blockIdx.x / (a.kv_heads * pa.splits);
     if (tid == 0) s_seq = 0xFFFFFFFFu;
-    uint32_t before = 0;
-    for (uint32_t b0 = 0; b0 < seqs; b0 += PP_THREADS) {
-        const uint32_t b = b0 + tid;
+    if (seqs <= PP_THREADS) {
         PgSeq mine = {};
-        if (b < seqs) mine = pg_seq(a, b);
-        const uint32_t n = b < seqs ? pp_blocks(pa, mine) : 0;
-        uint32_t incl = n;
+        uint32_t n = 0, before = 0;
+        if (tid < seqs) {
+            mine = pg_seq(a, tid);
+            n = pp_blocks(pa, mine);
+            s_kv[tid] = (uint64_t)mine.kv << 32 | n;
+        }
+        __syncthreads();
+        if (n) {
+#pragma unroll 8
+            for (uint32_t i = 0; i < seqs; i++) {
+                const uint64_t o = s_kv[i];
+                const uint32_t kv = (uint32_t)(o >> 32);
+                if (kv > mine.kv || (kv == mine.kv && i < tid)) before += (uint32_t)o;
+            }
+            if (before <= want && want - before < n) {
+                s_seq = tid;
+                s_before = before + n;
+                s_found = mine;
+            }
+        }
+        __syncthreads();
+    } else {
+        uint32_t* s_sum = reinterpret_cast<uint32_t*>(s_kv);
+        uint32_t before = 0;
+        for (uint32_t b0 = 0; b0 < seqs; b0 += PP_THREADS) {
+            const uint32_t b = b0 + tid;
+            PgSeq mine = {};
+            if (b < seqs) mine = pg_seq(a, b);
+            const uint32_t n = b < seqs ? pp_blocks(pa, mine) : 0;
+            uint32_t incl = n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-            if (lane >= (uint32_t)o) incl += t;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                if (lane >= (uint32_t)o) incl += t;
+            }
+            __syncthreads();
+            if (lane == 31) s_sum[warp] = incl;
+            __syncthreads();
+            uint32_t excl = before + incl - n;
+            for (uint32_t i = 0; i < PP_THREADS / 32; i++) {
+                if (i < warp) excl += s_sum[i];
+                before += s_sum[i];
+            }
+            if (excl <= want && want - excl < n) {
+                s_seq = b;
+                s_before = excl + n;
+                s_found = mine;
+            }
+            __syncthreads();
+            if (s_seq != 0xFFFFFFFFu) break;
         }
-        __syncthreads();
-        if (lane == 31) s_sum[warp] = incl;
-        __syncthreads();
-        uint32_t excl = before + incl - n;
-        for (uint32_t i = 0; i < PP_THREADS / 32; i++) {
-            if (i < warp) excl += s_sum[i];
-            before += s_sum[i];
-        }
-        if (excl <= want && want < excl + n) {
-            s_seq = b;
-            s_before = excl + n;
-            s_found = mine;
-        }
-        __syncthreads();
-        if (s_seq != 0xFFFFFFFFu) break;
     }
     if (s_seq == 0xFFFFFFFFu) {  // the grid is an upper bound (the same for all threads)
         if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0));
@@ -334,7 +363,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             pp_ld_done();
             const uint32_t key0 = t * PP_KEYS;
             if (SCORED) {
-                if (a.cap_mul != 0.0f || !a.slopes) {
+                if (a.cap_mul == 0.0f && !a.slopes) {
                     const uint64_t mul2 = pp_pack2(a.score_mul);
 #pragma unroll
                     for (uint32_t i = 0; i < 128; i += 2) pp_mul2(s[i], s[i + 1], mul2);
@@ -345,12 +374,15 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     for (uint32_t i = 0; i < 128; i += 8)
 #pragma unroll
                         for (uint32_t k = 0; k < 4; k++) far[k] = fmaxf(fmaxf(far[k], fabsf(s[i + k])), fabsf(s[i + 4 + k]));
-                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) <= 0.5f))) {
+                    const float b = a.score_mul;
+                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * fabsf(b) <= 0.5f))) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i], 1.0f);
+                        for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i] * b, 1.0f);
                     } else {
-                        const uint64_t k3 = pp_pack2(0.017005980014801025f), k2 = pp_pack2(-0.05292436107993126f), k1 = pp_pack2(0.13323938846588135f),
-                                       k0 = pp_pack2(-0.33333051204681396f), one = pp_pack2(1.0f);
+                        // tanh(b s) with b in the coefficients
+                        const float b2 = b * b;
+                        const uint64_t k3 = pp_pack2(0.017005980014801025f * b2 * b2 * b2 * b2 * b), k2 = pp_pack2(-0.05292436107993126f * b2 * b2 * b2 * b),
+                                       k1 = pp_pack2(0.13323938846588135f * b2 * b2 * b), k0 = pp_pack2(-0.33333051204681396f * b2 * b), one = pp_pack2(b);
 #pragma unroll
                         for (uint32_t i = 0; i < 128; i += 2) pp_tanh2(s[i], s[i + 1], k3, k2, k1, k0, one);
                     }
