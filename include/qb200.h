@@ -277,10 +277,10 @@ QB200_API qb200_status qb200_sum_arrays(const float* parts, uint32_t count, uint
  *   q_out NULL with heads = 0: keys and values alone.  A token whose place would be negative (more new tokens than
  *   keys) is not written.  Two tokens of one call must not have the same place.
  * qb200_paged_attention: token at place p of its sequence sees keys 0 .. p (causal), the first prefix_lens[b] keys
- *   too where prefix_lens is given, or all kv_lens[b] keys (causal = 0).  Score = scale * (q . k); softcap > 0: softcap *
+ *   too where prefix_lens is given, or all kv_lens[b] keys (causal = 0).  Score = scale * (q . k); softcap (0, or at least 1e-6) > 0: softcap *
  *   tanh(score / softcap); slopes [heads] given: minus slopes[h] * |distance|.  heads is a multiple of kv_heads, head h
  *   reads K/V head h / (heads / kv_heads).  q [tokens, heads * head_dim] of the cache's type (rows q_stride elements
- *   apart, a multiple of 8; 16-byte aligned), out [tokens, heads * head_dim] dense; lse [tokens, heads] f32 or NULL: log of the sum of
+ *   apart, a multiple of 8; 16-byte aligned), out [tokens, heads * head_dim] dense, not overlapping q; lse [tokens, heads] f32 or NULL: log of the sum of
  *   exp(score).  A row that sees no key gives zeros and -inf.  f32 softmax and accumulation; the softmax weights enter the second
  *   product in the cache's type.  scratch: qb200_paged_attention_scratch_floats floats, 16-byte aligned, not shared with
  *   a call that may overlap.  A key or value of a sequence that is not finite reaches every row that is computed in

@@ -200,8 +200,9 @@ static qb200_status pg_check_attention(const char* who, const qb200_paged_kv* kv
     if (q_stride < (uint64_t)heads * kv->head_dim || q_stride % 8) return fail(QB200_ERR_LENGTH, w + ": q's row stride must be a multiple of 8 that holds all heads");
     if (!pg_aligned(q, 16) || !pg_aligned(out, 16) || !pg_aligned(scratch, 16))
         return fail(QB200_ERR_INVALID_PARAM, w + ": q, out and scratch must be 16-byte aligned");
-    if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f)
-        return fail(QB200_ERR_INVALID_PARAM, w + ": the scale must be finite and the cap finite and not negative");
+    if (!std::isfinite(scale) || !std::isfinite(softcap) || (softcap != 0.0f && softcap < 1e-6f))
+        return fail(QB200_ERR_INVALID_PARAM, w + ": the scale must be finite, and the cap finite and 0 or at least 1e-6");
+    if (tokens && q == out) return fail(QB200_ERR_INVALID_PARAM, w + ": the output must not overlap q");
     return QB200_OK;
 }
 

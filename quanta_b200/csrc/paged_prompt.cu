@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
 #pragma unroll
                         for (uint32_t k = 0; k < 4; k++) far[k] = fmaxf(fmaxf(far[k], fabsf(s[i + k])), fabsf(s[i + 4 + k]));
                     const float b = a.score_mul;
-                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * fabsf(b) <= 0.5f))) {
+                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * fabsf(b) <= 0.5f && fabsf(b) <= 64.0f))) {  // (b^9 stays in range)
 #pragma unroll
                         for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i] * b, 1.0f);
                     } else {

@@ -105,6 +105,80 @@ def test_rows_and_sequences_that_see_nothing():
     run(8, [1, 130], [0, 5], 8, 1, prefix=19)
 
 
+def wide_run(q_lens, kv_lens, heads, kv_heads, hd, dtype, ps=16, width=4096, **kw):
+    """As run(), with a table far wider than the sequences need: the lengths' upper bound decides how the work is cut."""
+    m = ref.make(77, q_lens, kv_lens, heads, kv_heads, hd, ps, dtype)
+    cache = paged.PagedKVCache.from_parts(m["k"].to(DEV), m["v"].to(DEV))
+    table = torch.full((len(kv_lens), width), -3, dtype=torch.int32)
+    table[:, : m["table"].shape[1]] = m["table"]
+    batch = paged.PagedBatch(cache, table.to(DEV), ints(kv_lens), ints(m["cu"]))
+    out = paged.paged_attention(batch, m["q"].to(DEV), **kw)
+    cache.check()
+    want, _, tol, _ = ref.attention(m["q"], m["k"], m["v"], m["table"], kv_lens, m["cu"], heads, 1.0 / math.sqrt(hd), kw.get("softcap", 0.0))
+    within(out, want, tol)
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, BF), (64, FP)])
+def test_many_short_sequences_in_wide_tables(hd, dtype):
+    """Several units in one CTA's run, units cut by run ends, more sequences than a CTA keeps lengths of, empty ones between."""
+    g = torch.Generator().manual_seed(3)
+    kv = torch.randint(1, 200, (170,), generator=g).tolist()
+    q = [1] * 170
+    for i in (0, 17, 127, 128, 129, 169):
+        q[i] = kv[i] = 0
+    for i in (5, 60, 140):
+        q[i] = min(3, kv[i])
+    wide_run(q, kv, 8, 4, hd, dtype)
+    wide_run([1, 1, 0, 1], [2900, 1, 40, 700], 4, 1, hd, dtype)
+    wide_run([1], [1], 4, 4, hd, dtype, softcap=2.0)
+
+
+def test_more_sequences_than_a_block_has_threads():
+    """Prompts among many single tokens: the prompt kernel's search over a long batch."""
+    q, kv = [1] * 430, [1 + i % 7 for i in range(430)]
+    for i, (a, b) in {3: (40, 50), 200: (0, 0), 399: (70, 70), 400: (33, 90), 429: (20, 20)}.items():
+        q[i], kv[i] = a, b
+    run(13, q, kv, 2, 1, 64, 16, FP)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [700, 90]), ([300], [700])])
+@pytest.mark.parametrize("rising", [True, False])
+def test_scores_that_rise_and_fall_along_the_keys(q_lens, kv_lens, rising):
+    """The running maximum moves in every tile, or never after the first; scores of several hundred, one key wins."""
+    m = ref.make(5, q_lens, kv_lens, 2, 1, 128, 16, BF)
+    for b, n in enumerate(kv_lens):
+        for j in range(n):
+            x = (j if rising else n - j) / n
+            m["k"][int(m["table"][b, j // 16]), :, j % 16] = (m["k"][int(m["table"][b, j // 16]), :, j % 16].float() * 0.05 + 4.0 * x).to(BF)
+    m["q"] = (m["q"].float().abs() + 0.5).to(BF)
+    cache, batch = build(m, kv_lens)
+    out = paged.paged_attention(batch, m["q"].to(DEV))
+    cache.check()
+    want, _, tol, _ = ref.attention(m["q"], m["k"], m["v"], m["table"], kv_lens, m["cu"], 2, 1.0 / math.sqrt(128))
+    within(out, want, tol)
+
+
+def test_two_calls_at_once():
+    """Prompts and single tokens over the same cache and batch from two streams."""
+    m = ref.make(90, [260, 1, 30], [600, 900, 200], 8, 2, 128, 16, BF, garbage=0.25)
+    cache, batch = build(m, [600, 900, 200])
+    ones = paged.PagedBatch(cache, batch.table, batch.kv_lens)
+    q, q1 = m["q"].to(DEV), torch.randn(3, 1024, device=DEV).to(BF)
+    want, want1 = paged.paged_attention(batch, q), paged.paged_attention(ones, q1)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    a.wait_stream(torch.cuda.current_stream())
+    b.wait_stream(torch.cuda.current_stream())
+    got, got1 = [], []
+    for _ in range(20):
+        with torch.cuda.stream(a):
+            got.append(paged.paged_attention(batch, q))
+        with torch.cuda.stream(b):
+            got1.append(paged.paged_attention(ones, q1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got) and all(torch.equal(x, want1) for x in got1)
+    cache.check()
+
+
 def test_long_keys_and_few_sequences():
     """One sequence over every SM: its keys are cut into many runs that are joined."""
     run(9, [1], [5003], 4, 2, ragged=False)

@@ -27,12 +27,12 @@ def seqs(**kw):
     return L.PagedBatch(**d)
 
 
-def attend(c=None, b=None, q=P, q_stride=512, tokens=5, heads=4, scale=0.1, cap=0.0, scratch=P, out=P):
+def attend(c=None, b=None, q=P, q_stride=512, tokens=5, heads=4, scale=0.1, cap=0.0, scratch=P, out=2 * P):
     return lib.qb200_paged_attention(ctypes.byref(c or kv()), ctypes.byref(b or seqs()), q, q_stride, tokens, heads, scale, cap, None, None, 1, scratch, out, None, None)
 
 
-def prefix(c=None, b=None, pages=P, n=20, q=P, tokens=5, heads=4, cap=0.0):
-    return lib.qb200_shared_prefix_attention(ctypes.byref(c or kv()), ctypes.byref(b or seqs()), pages, n, q, 512, tokens, heads, 0.1, cap, None, P, P, None, None)
+def prefix(c=None, b=None, pages=P, n=20, q=P, tokens=5, heads=4, cap=0.0, out=2 * P):
+    return lib.qb200_shared_prefix_attention(ctypes.byref(c or kv()), ctypes.byref(b or seqs()), pages, n, q, 512, tokens, heads, 0.1, cap, None, P, out, None, None)
 
 
 def append(c=None, b=None, q=P, k=P, v=P, dt=L.F32, qs=512, ks=256, vs=256, tokens=5, heads=4, cos=P, sin=P, rot=128, n_pos=9, q_out=P):
@@ -60,8 +60,8 @@ def test_attention_refusals():
         assert f(heads=3) == L.ERR_INVALID_PARAM and "multiple" in L.last_error()
         assert f(heads=0) == L.ERR_INVALID_PARAM
         assert f(q=None) == L.ERR_INVALID_PARAM
-        assert f(q=P + 2) == L.ERR_INVALID_PARAM
-        assert f(cap=-1.0) == L.ERR_INVALID_PARAM and f(cap=float("inf")) == L.ERR_INVALID_PARAM
+        assert f(q=P + 2) == L.ERR_INVALID_PARAM and f(out=P) == L.ERR_INVALID_PARAM
+        assert f(cap=-1.0) == L.ERR_INVALID_PARAM and f(cap=float("inf")) == L.ERR_INVALID_PARAM and f(cap=1e-9) == L.ERR_INVALID_PARAM
         assert f(tokens=1 << 28) == L.ERR_NOT_SUPPORTED
     assert attend(q_stride=500) == L.ERR_LENGTH and attend(q_stride=516) == L.ERR_LENGTH
     assert attend(scale=float("nan")) == L.ERR_INVALID_PARAM
