@@ -193,7 +193,7 @@ static qb200_status pg_check_attention(const char* who, const qb200_paged_kv* kv
     qb200_status st = pg_check_cache(who, kv, b, tokens);
     if (st) return st;
     const std::string w(who);
-    if (tokens && (!q || !out || !scratch)) return fail(QB200_ERR_INVALID_PARAM, w + ": null pointer");
+    if (tokens && (!q || !out)) return fail(QB200_ERR_INVALID_PARAM, w + ": null pointer");
     if (heads == 0 || heads % kv->kv_heads)
         return fail(QB200_ERR_INVALID_PARAM, w + ": " + std::to_string(heads) + " heads are no multiple of " + std::to_string(kv->kv_heads) + " K/V heads");
     if (tokens * heads > 0x7FFFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, w + ": 2^31 query rows or more");
@@ -247,10 +247,18 @@ static PgPlan pg_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
     PgPlan p = {};
     const uint64_t most = a.shared || a.cu_q ? (uint64_t)a.tokens * a.group : a.group;
     p.many = most > PG_FEW_ROWS;
+    if (p.many && most <= PG_FEW_IN_ALL) {
+        p.rows = pg_rows_plan(a, hd, sms, (uint32_t)div_ceil(most, PG_FEW_ROWS));
+        if (p.rows.units) {
+            p.few = true;
+            p.many = false;
+            return p;
+        }
+    }
     p.few = !p.many || (!a.shared && a.cu_q && a.group <= PG_FEW_ROWS);
     p.min_rows = p.few ? PG_FEW_ROWS + 1 : 1;
     if (p.few) {
-        p.rows = pg_rows_plan(a, hd, sms);
+        p.rows = pg_rows_plan(a, hd, sms, 1);
         p.floats = p.rows.floats;
     }
     if (p.many) {
@@ -259,12 +267,12 @@ static PgPlan pg_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
         if (n > p.floats) p.floats = n;
     }
     p.floats = (p.floats + 3) / 4 * 4;
-    if (!p.floats) p.floats = 4;
     return p;
 }
 
-static qb200_status pg_phase(PgArgs a, int dtype, uint32_t hd, uint32_t sms, float* scratch, cudaStream_t st) {
+static qb200_status pg_phase(const char* who, PgArgs a, int dtype, uint32_t hd, uint32_t sms, float* scratch, cudaStream_t st) {
     const PgPlan p = pg_plan(a, hd, sms);
+    if (p.floats && !scratch) return fail(QB200_ERR_INVALID_PARAM, std::string(who) + ": the call needs its scratch");
     if (p.many) {
         a.parts = scratch;
         const qb200_status r = pg_prompt_launch(a, dtype, hd, p.splits, p.min_rows, st);
@@ -385,7 +393,7 @@ qb200_status qb200_paged_attention(const qb200_paged_kv* kv, const qb200_paged_b
     a.out = static_cast<uint16_t*>(out);
     a.lse = lse;
     pg_scores(a, scale, softcap, slopes);
-    return pg_phase(a, kv->dtype, kv->head_dim, sms, scratch, static_cast<cudaStream_t>(stream));
+    return pg_phase("qb200_paged_attention", a, kv->dtype, kv->head_dim, sms, scratch, static_cast<cudaStream_t>(stream));
 }
 
 // The prefix phase leaves the state (m, l, acc) of every row in 32 bits; the phase over the sequences' own keys joins it
@@ -430,14 +438,15 @@ qb200_status qb200_shared_prefix_attention(const qb200_paged_kv* kv, const qb200
     a.q = q;
     a.q_stride = q_stride;
     pg_scores(a, scale, softcap, slopes);
+    if (!scratch) return fail(QB200_ERR_INVALID_PARAM, std::string(who) + ": the call needs its scratch");
     float* phase = scratch + prefix_rows_floats(a, kv->head_dim);
     const PgArgs p = prefix_args(a, prefix_pages, prefix_len, kv->head_dim, scratch);
-    if ((st = pg_phase(p, kv->dtype, kv->head_dim, sms, phase, s))) return st;
+    if ((st = pg_phase(who, p, kv->dtype, kv->head_dim, sms, phase, s))) return st;
     a.base_acc = p.rows_acc;
     a.base_ml = p.rows_ml;
     a.out = static_cast<uint16_t*>(out);
     a.lse = lse;
-    return pg_phase(a, kv->dtype, kv->head_dim, sms, phase, s);
+    return pg_phase(who, a, kv->dtype, kv->head_dim, sms, phase, s);
 }
 
 qb200_status qb200_paged_check(const qb200_paged_kv* kv, void* stream) {

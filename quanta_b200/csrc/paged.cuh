@@ -17,8 +17,9 @@
 
 namespace qb {
 
-// Sequences of at most this many packed rows go to the kernel for few rows, the others to the prompt kernel.
-constexpr uint32_t PG_FEW_ROWS = 16;
+// Sequences of at most this many packed rows go to the kernels for few rows, the others to the prompt kernel; calls of at
+// most PG_FEW_IN_ALL rows a K/V head go to the former as a whole where their tables are of moderate length.
+constexpr uint32_t PG_FEW_ROWS = 16, PG_FEW_IN_ALL = 64;
 
 constexpr float PG_LOG2E = 1.4426950408889634f, PG_LN2 = 0.6931471805599453f;
 
@@ -209,12 +210,12 @@ __device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_
 
 // Attention for few rows (paged_rows.cu): how it runs and the floats of partial results that takes.
 struct PgRows {
-    bool units;      // a cluster of 2^c_log CTAs per unit; otherwise equal runs of all tiles, and a second kernel
-    uint32_t c_log, grid;
+    bool units;      // a cluster of 2^c_log CTAs per unit of 16 rows, row_tiles of them a sequence and K/V head; otherwise equal runs of all tiles, and a second kernel
+    uint32_t c_log, grid, row_tiles;
     uint64_t floats;
 };
 uint64_t pg_rows_most_tiles(const PgArgs& a);  // below 2^32, or the call is refused
-PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms);
+PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms, uint32_t row_tiles);
 qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, const PgRows& how, cudaStream_t st);
 // Attention for many rows (paged_prompt.cu): over how many ranges a unit's keys are cut, the floats of partial results
 // that takes, and the launch; min_rows: sequences of fewer packed rows are not its own.

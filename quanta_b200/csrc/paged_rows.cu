@@ -168,10 +168,10 @@ template <uint32_t HD> struct PrState {
     int32_t pos[2];
 };
 template <uint32_t HD, bool SCORED>
-__device__ __forceinline__ void pr_begin(const PgArgs& a, const PgSeq& sq, uint32_t kvh, PrState<HD>& u) {
+__device__ __forceinline__ void pr_begin(const PgArgs& a, const PgSeq& sq, uint32_t kvh, uint32_t row0, PrState<HD>& u) {
 #pragma unroll
     for (uint32_t i = 0; i < 2; i++) {
-        const uint32_t r = ((threadIdx.x & 31) >> 2) + 8 * i;
+        const uint32_t r = row0 + ((threadIdx.x & 31) >> 2) + 8 * i;
         u.m[i] = -INFINITY;
         u.l[i] = 0.0f;
         u.lim[i] = 0;
@@ -188,10 +188,10 @@ __device__ __forceinline__ void pr_begin(const PgArgs& a, const PgSeq& sq, uint3
 #pragma unroll
     for (uint32_t k = 0; k < HD / 8; k++) u.o[k][0] = u.o[k][1] = u.o[k][2] = u.o[k][3] = 0.0f;
 }
-// A 16-byte chunk of the unit's 16 rows of Q (zeros past the last row).
+// A 16-byte chunk of the unit's 16 rows of Q, from row0 on (zeros past the last row).
 template <uint32_t HD>
-__device__ __forceinline__ uint4 pr_load_q(const PgArgs& a, const PgSeq& sq, uint32_t kvh, uint32_t id) {
-    const uint32_t r = id / (HD / 8), c = id % (HD / 8);
+__device__ __forceinline__ uint4 pr_load_q(const PgArgs& a, const PgSeq& sq, uint32_t kvh, uint32_t row0, uint32_t id) {
+    const uint32_t r = row0 + id / (HD / 8), c = id % (HD / 8);
     if (r >= sq.q_len * a.group) return make_uint4(0, 0, 0, 0);
     return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (uint64_t)(sq.q0 + r / a.group) * a.q_stride +
                                            (uint64_t)(kvh * a.group + r % a.group) * HD + c * 8);
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
     uint4 q_in[QN];
     auto bring_q = [&](const PrAt& p) {
 #pragma unroll
-        for (uint32_t i = 0; i < QN; i++) q_in[i] = pr_load_q<HD>(a, p.s, p.kvh, i * 128 + tid);
+        for (uint32_t i = 0; i < QN; i++) q_in[i] = pr_load_q<HD>(a, p.s, p.kvh, 0, i * 128 + tid);
     };
 
     bring_q(here);
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
         const uint32_t kvh = here.kvh, rows = sq.q_len * a.group, t0 = here.t, n = min(here.tiles - t0, here.left);
         const bool whole = n == here.tiles;
         PrState<HD> u;
-        pr_begin<HD, SCORED>(a, sq, kvh, u);
+        pr_begin<HD, SCORED>(a, sq, kvh, 0, u);
 
         for (uint32_t t = t0; t < t0 + n; t++) {
             pr_wait<S::STAGES - 2>();
@@ -478,34 +478,38 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
 }
 
 // The same for tables of moderate length, in one launch and without a search: a unit has a cluster of 2^c_log CTAs, each
-// takes an equal range of its tiles, and their states meet in the cluster's shared memory.
+// takes an equal range of its tiles, and their states meet in the cluster's shared memory.  Where the call has few rows in
+// all, sequences of up to row_tiles * 16 rows are taken, 16 rows a unit (side by side, so that they share the L2).
 template <typename T, uint32_t HD, bool SCORED>
-__global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_constant__ PgArgs a, uint32_t c_log) {
+__global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_constant__ PgArgs a, uint32_t c_log, uint32_t row_tiles) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     using S = PrShape<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5;
-    const uint32_t rank = blockIdx.x & ((1u << c_log) - 1), unit = blockIdx.x >> c_log, b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
+    const uint32_t rank = blockIdx.x & ((1u << c_log) - 1), unit = blockIdx.x >> c_log, b = unit / (a.kv_heads * row_tiles);
+    const uint32_t in = unit - b * a.kv_heads * row_tiles, kvh = in / row_tiles, row0 = (in - kvh * row_tiles) * PR_ROWS;
     const PgSeq sq = pg_seq(a, b);
-    const uint32_t rows = sq.q_len * a.group;
-    if (rows == 0 || rows > PG_FEW_ROWS) return;  // the whole cluster alike
+    const uint32_t all_rows = sq.q_len * a.group;
+    if (all_rows <= row0 || all_rows > row_tiles * PR_ROWS) return;  // the whole cluster alike
+    const uint32_t rows = min(PR_ROWS, all_rows - row0);
+    const uint32_t keys = pg_limit(sq, (row0 + rows - 1) / a.group);  // that the unit's last token sees (the most)
     const uint32_t ring_s = pr_smem(smem + warp * S::WARP), q_s = pr_smem(smem + S::Q);
     float* j_acc = reinterpret_cast<float*>(smem + S::JOIN);
     float* j_ml = reinterpret_cast<float*>(smem + S::ML);
     const uint64_t once = pr_once();
-    const uint32_t tiles = pr_tiles(sq), t0 = tiles * rank >> c_log, t1 = tiles * (rank + 1) >> c_log;
+    const uint32_t tiles = max(1u, (keys + PR_TILE - 1) / PR_TILE), t0 = tiles * rank >> c_log, t1 = tiles * (rank + 1) >> c_log;
     const int32_t* table = a.table + (a.shared ? 0 : (uint64_t)b * a.table_stride);
     uint32_t ahead = t0;  // the next tile to fetch, and its page
     int32_t page = 0;
     auto look = [&]() {
         const uint32_t key = ahead * PR_TILE + warp * PR_KEYS;
-        if (ahead < t1 && key < sq.kv) page = table[key >> a.ps_log];
+        if (ahead < t1 && key < keys) page = table[key >> a.ps_log];
     };
     auto fetch = [&](uint32_t st) {
         if (ahead < t1) {
             const uint32_t key = ahead * PR_TILE + warp * PR_KEYS;
-            pr_copy_keys<HD>(a, ring_s + st * S::STAGE, page, kvh, key, key < sq.kv ? min(sq.kv - key, PR_KEYS) : 0, once);
+            pr_copy_keys<HD>(a, ring_s + st * S::STAGE, page, kvh, key, key < keys ? min(keys - key, PR_KEYS) : 0, once);
             ahead++;
             look();
         }
@@ -514,7 +518,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_c
     constexpr uint32_t QN = PR_ROWS * (HD / 8) / 128;
     uint4 q_in[QN];
 #pragma unroll
-    for (uint32_t i = 0; i < QN; i++) q_in[i] = pr_load_q<HD>(a, sq, kvh, i * 128 + tid);
+    for (uint32_t i = 0; i < QN; i++) q_in[i] = pr_load_q<HD>(a, sq, kvh, row0, i * 128 + tid);
     look();
 #pragma unroll
     for (uint32_t i = 0; i + 1 < S::STAGES; i++) fetch(i);
@@ -524,7 +528,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_c
     uint32_t qf[HD / 16][4];
     pr_q_fragments<HD>(q_s, qf);
     PrState<HD> u;
-    pr_begin<HD, SCORED>(a, sq, kvh, u);
+    pr_begin<HD, SCORED>(a, sq, kvh, row0, u);
     uint32_t st = 0;
     for (uint32_t t = t0; t < t1; t++) {
         pr_wait<S::STAGES - 2>();
@@ -549,7 +553,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_c
             float M, L;
             const float4 v = pr_join_warps<HD>(j_acc, j_ml, r, p0, col, M, L);
             if (c_log == 0) {
-                pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
+                pg_emit<T, HD>(a, sq.q0 + (row0 + r) / a.group, kvh * a.group + (row0 + r) % a.group, col, M, L, v);
                 continue;
             }
             *reinterpret_cast<float4*>(mine + r * ROW + 4 + col) = v;
@@ -590,7 +594,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_c
             v.z = fmaf(e[p].z, g, v.z);
             v.w = fmaf(e[p].w, g, v.w);
         }
-        pg_emit<T, HD>(a, sq.q0 + r / a.group, kvh * a.group + r % a.group, col, M, L, v);
+        pg_emit<T, HD>(a, sq.q0 + (row0 + r) / a.group, kvh * a.group + (row0 + r) % a.group, col, M, L, v);
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // no CTA leaves while its state is read
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -687,9 +691,10 @@ uint64_t pg_rows_most_tiles(const PgArgs& a) {
     return (a.shared ? 1 : (uint64_t)a.batch) * a.kv_heads * div_ceil(keys, PR_TILE);
 }
 
-PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
+PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms, uint32_t row_tiles) {
     PgRows how = {};
-    const uint64_t most = pg_rows_most_tiles(a), units = (a.shared ? 1 : (uint64_t)a.batch) * a.kv_heads, tiles = most / units;
+    how.row_tiles = row_tiles;
+    const uint64_t most = pg_rows_most_tiles(a), seqs = (a.shared ? 1 : (uint64_t)a.batch) * a.kv_heads, units = seqs * row_tiles, tiles = most / seqs;
     // A cluster per unit, of up to 8 CTAs while all of them fit the SMs at once, where a CTA then has at most PR_SHORT
     // tiles, or at most PR_LONG and there are as many CTAs as SMs; equal runs otherwise.
     uint32_t c_log = 0;
@@ -700,6 +705,7 @@ PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms) {
         how.grid = (uint32_t)(units << c_log);
         return how;
     }
+    if (row_tiles > 1) return how;  // the equal runs take one tile of rows
     how.grid = (uint32_t)(most < 2 * sms ? most : 2 * sms);  // two CTAs per SM, fewer where the call cannot have as many tiles
     how.floats = (uint64_t)how.grid * 2 * PR_ROWS * (hd + 2) + (uint64_t)how.grid * 8;
     return how;
@@ -717,7 +723,7 @@ static qb200_status launch_rows(const PgArgs& a, const PgRows& how, cudaStream_t
     }
     const uint32_t grid = how.grid;
     if (how.units) {
-        QB_CUDA_TRY(pg_launch_cluster(k_paged_units<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, 1u << how.c_log, a, how.c_log));
+        QB_CUDA_TRY(pg_launch_cluster(k_paged_units<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, 1u << how.c_log, a, how.c_log, how.row_tiles));
         return QB200_OK;
     }
     QB_CUDA_TRY(pg_launch(k_paged_rows<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, a));

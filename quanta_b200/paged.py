@@ -185,9 +185,9 @@ def _attend(who: str, batch: PagedBatch, q: torch.Tensor, slopes, out, lse):
     return tokens, heads, qs, 0 if slopes is None else _small(slopes, torch.float32, heads, dev, who + ": slopes"), out, 0 if lse is None else lse.data_ptr()
 
 
-def _scratch(who: str, batch: PagedBatch, scratch: Optional[torch.Tensor], size_of, *shape) -> torch.Tensor:
+def _scratch(who: str, batch: PagedBatch, scratch: Optional[torch.Tensor], size_of, *shape) -> Optional[torch.Tensor]:
     """The call's workspace: the caller's, or one of its own from torch's allocator (which keeps calls on different
-    streams and in different captured graphs apart)."""
+    streams and in different captured graphs apart), or None where it needs none."""
     cache = batch.cache
     floats = batch._floats.get(shape)
     if floats is None:
@@ -198,7 +198,7 @@ def _scratch(who: str, batch: PagedBatch, scratch: Optional[torch.Tensor], size_
         with torch.cuda.device(cache._index):
             floats = batch._floats[shape] = size_of(cache._ref, batch._ref, *shape)
     if scratch is None:
-        return cache._f32.new_empty(floats)
+        return cache._f32.new_empty(floats) if floats else None
     if scratch.dtype != torch.float32 or scratch.device != cache.device or not scratch.is_contiguous() or scratch.numel() < floats:
         _bad(f"{who}: scratch must be {floats} contiguous f32 values on {cache.device}", L.ERR_LENGTH)
     return scratch
@@ -218,7 +218,7 @@ def paged_attention(batch: PagedBatch, q: torch.Tensor, scale: Optional[float] =
     lib = L.load()
     scratch = _scratch("paged_attention", batch, scratch, lib.qb200_paged_attention_scratch_floats, tokens, heads)
     _run(cache, lib.qb200_paged_attention, cache._ref, batch._ref, q.data_ptr(), qs, tokens, heads, cache._scale if scale is None else scale, softcap, sl, pl,
-         1 if causal else 0, scratch.data_ptr(), out.data_ptr(), lp)
+         1 if causal else 0, 0 if scratch is None else scratch.data_ptr(), out.data_ptr(), lp)
     return out
 
 

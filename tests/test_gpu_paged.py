@@ -436,7 +436,8 @@ def test_python_refusals_on_the_device():
                  lambda: paged.paged_attention(batch, q, softcap=-1.0), lambda: paged.paged_attention(batch, q, scale=float("nan")),
                  lambda: paged.paged_attention(batch, q, slopes=one[:3]), lambda: paged.paged_attention(batch, q, slopes=one.double()),
                  lambda: paged.paged_attention(batch, q, prefix_lens=ints([1])), lambda: paged.paged_attention(batch, q, out=q[:1]),
-                 lambda: paged.paged_attention(batch, q, lse=one), lambda: paged.paged_attention(batch, q, scratch=one[:1]),
+                 lambda: paged.paged_attention(batch, q, lse=one), lambda: paged.paged_attention(batch, q, scratch=one.double()),
+                 lambda: paged.shared_prefix_attention(batch, q, ints([1]), 16, scratch=one),
                  lambda: paged.shared_prefix_attention(batch, q, ints([1]), 17), lambda: paged.shared_prefix_attention(batch, q, ints([1]), 0),
                  lambda: paged.paged_rope_append(batch, q, q[:, :256], q[:, :128], one, one),
                  lambda: paged.paged_rope_append(batch, q, q[:, :256], q[:, :256], one.reshape(2, 2), one.reshape(1, 4)),

@@ -65,7 +65,7 @@ def test_attention_refusals():
         assert f(tokens=1 << 28) == L.ERR_NOT_SUPPORTED
     assert attend(q_stride=500) == L.ERR_LENGTH and attend(q_stride=516) == L.ERR_LENGTH
     assert attend(scale=float("nan")) == L.ERR_INVALID_PARAM
-    assert attend(out=None) == L.ERR_INVALID_PARAM and attend(scratch=None) == L.ERR_INVALID_PARAM and attend(out=P + 4) == L.ERR_INVALID_PARAM
+    assert attend(out=None) == L.ERR_INVALID_PARAM and attend(scratch=P + 4) == L.ERR_INVALID_PARAM and attend(out=P + 4) == L.ERR_INVALID_PARAM
     assert prefix(n=0) == L.ERR_INVALID_PARAM and prefix(pages=None) == L.ERR_INVALID_PARAM and prefix(n=1 << 31) == L.ERR_NOT_SUPPORTED
     assert attend(tokens=0) == L.OK and prefix(tokens=0) == L.OK  # nothing to do
 
