@@ -18,8 +18,8 @@
 namespace qb {
 
 // Sequences of at most this many packed rows go to the kernels for few rows, the others to the prompt kernel; calls of at
-// most PG_FEW_IN_ALL rows a K/V head go to the former as a whole where their tables are of moderate length.
-constexpr uint32_t PG_FEW_ROWS = 16, PG_FEW_IN_ALL = 64;
+// most PG_FEW_IN_ALL rows a K/V head go to the former as a whole where that is little work (pg_rows_plan).
+constexpr uint32_t PG_FEW_ROWS = 16, PG_FEW_IN_ALL = 1024;
 
 constexpr float PG_LOG2E = 1.4426950408889634f, PG_LN2 = 0.6931471805599453f;
 

@@ -71,6 +71,10 @@ __device__ __forceinline__ uint32_t pr_weight(const PgArgs& a, const PgSeq& s) {
 // by clusters / by runs, K/V heads x sequences x keys: 8 x 1 x 1024 5.1 / 7.1, 8 x 1 x 4096 8.8 / 10.6, 8 x 1 x 16384 25 / 19;
 // 32 x 16 x 1024 42 / 46, 8 x 64 x 2048 80 / 84 (lengths up to 2048: 51 / 54), 8 x 64 x 8192 301 / 313 (up to 8192: 190 / 172).
 constexpr uint32_t PR_SHORT = 8, PR_LONG = 32;
+// Steps (16 rows against 64 keys of a K/V head) up to which a call of several row tiles stays here, us here / by the prompt
+// kernel: 8 K/V heads, 512 rows, 128 keys 6.6 / 10.4; 128 rows, 1000 keys 9.5 / 15.2; 64 tokens of 4 heads behind 1000
+// shared keys (2048 steps) 19.8 / 22.4, behind 4000 (8064 steps) 39 / 28.
+constexpr uint64_t PR_STEPS = 6144;
 
 // Sequences whose lengths the CTA keeps in shared memory: the first ones of the call.
 constexpr uint32_t PR_KEPT = PR_WARPS * 32;
@@ -699,6 +703,7 @@ PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms, uint32_t row_til
     // tiles, or at most PR_LONG and there are as many CTAs as SMs; equal runs otherwise.
     uint32_t c_log = 0;
     while (c_log < 3 && (units << (c_log + 1)) <= 2 * sms && (2u << c_log) <= tiles) c_log++;
+    if (row_tiles > 1 && most * row_tiles > PR_STEPS) return how;
     if (units <= 0x7FFFFFFFull >> c_log && (tiles <= (uint64_t)PR_SHORT << c_log || (tiles <= (uint64_t)PR_LONG << c_log && units << c_log >= sms))) {
         how.units = true;
         how.c_log = c_log;

@@ -80,9 +80,9 @@ def rotate(x, cos, sin):
     return y, 2 * 2.0 ** -24 * mag  # two products and a sum in 32 bits
 
 
-def make(seed, q_lens, kv_lens, heads, kv_heads, hd, ps, dtype, garbage=float("nan"), prefix=0, spare=2, tail=0):
+def make(seed, q_lens, kv_lens, heads, kv_heads, hd, ps, dtype, garbage=float("nan"), prefix=0, spare=2, tail=0, width=0):
     """Pools, table and queries on the CPU; pages in a random order, `garbage` wherever no sequence has a key; `tail` rows
-    of q belong to nobody."""
+    of q belong to nobody; the table has at least `width` columns."""
     g = torch.Generator().manual_seed(seed)
     need = [-(-n // ps) for n in kv_lens]
     n_pre = -(-prefix // ps)
@@ -90,7 +90,7 @@ def make(seed, q_lens, kv_lens, heads, kv_heads, hd, ps, dtype, garbage=float("n
     k = torch.randn(n_pages, kv_heads, ps, hd, generator=g).to(dtype)
     v = torch.randn(n_pages, kv_heads, ps, hd, generator=g).to(dtype)
     perm = torch.randperm(n_pages, generator=g).to(torch.int32)
-    table = torch.full((len(kv_lens), max(need) + 1), -7, dtype=torch.int32)
+    table = torch.full((len(kv_lens), max(width, max(need) + 1)), -7, dtype=torch.int32)
     used = torch.zeros(n_pages, ps, dtype=torch.bool)
     at = 0
     for b, n in enumerate(kv_lens):

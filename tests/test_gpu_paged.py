@@ -14,6 +14,11 @@ DEV = "cuda:0"
 BF, FP = torch.bfloat16, torch.float16
 
 
+# A table that could hold this many pages a sequence: the lengths' upper bound is what decides which kernel a call takes, so
+# short sequences in wide tables reach the kernels that long ones would.
+WIDE = 2500
+
+
 def ints(x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
@@ -34,8 +39,8 @@ def within(got, want, tol, rows=None):
 
 
 def run(seed, q_lens, kv_lens, heads, kv_heads, hd=128, ps=16, dtype=BF, tail=0, prefix=0, cap=0.0, slopes=False, prefix_lens=None, causal=True, scale=None,
-        ragged=True, garbage=float("nan")):
-    m = ref.make(seed, q_lens, kv_lens, heads, kv_heads, hd, ps, dtype, garbage, prefix, tail=tail)
+        ragged=True, garbage=float("nan"), width=0):
+    m = ref.make(seed, q_lens, kv_lens, heads, kv_heads, hd, ps, dtype, garbage, prefix, tail=tail, width=width)
     sc = 1.0 / math.sqrt(hd) if scale is None else scale
     sl = torch.tensor([2.0 ** (-8.0 * (h + 1) / heads) for h in range(heads)], dtype=torch.float32) if slopes else None
     cache, batch = build(m, kv_lens, ragged)
@@ -65,14 +70,16 @@ def run(seed, q_lens, kv_lens, heads, kv_heads, hd=128, ps=16, dtype=BF, tail=0,
 def test_single_tokens(heads, kv_heads, dtype, hd):
     """One new token per sequence, from one key to several tiles, with and without explicit row starts."""
     kv = [1, 2, 15, 16, 17, 63, 64, 65, 130, 257]
-    run(heads + hd, [1] * len(kv), kv, heads, kv_heads, hd, 16, dtype, ragged=False)
+    for width in (0, WIDE):
+        run(heads + hd, [1] * len(kv), kv, heads, kv_heads, hd, 16, dtype, ragged=False, width=width)
     run(heads + hd + 1, [1] * len(kv), kv, heads, kv_heads, hd, 32, dtype, tail=3)
 
 
+@pytest.mark.parametrize("width", [0, WIDE])
 @pytest.mark.parametrize("ps", [16, 32, 64, 128, 256])
-def test_page_sizes(ps):
-    run(ps, [1, 1, 1, 5], [ps - 1, ps, ps + 1, 3 * ps + 7], 8, 2, ps=ps)
-    run(ps + 1, [70, 33], [ps + 70, 333], 8, 2, ps=ps, dtype=FP, hd=64)
+def test_page_sizes(ps, width):
+    run(ps, [1, 1, 1, 5], [ps - 1, ps, ps + 1, 3 * ps + 7], 8, 2, ps=ps, width=width)
+    run(ps + 1, [70, 33], [ps + 70, 333], 8, 2, ps=ps, dtype=FP, hd=64, width=width)
 
 
 @pytest.mark.parametrize("dtype,hd", [(BF, 128), (FP, 128), (BF, 64), (FP, 64)])
@@ -83,7 +90,8 @@ def test_page_sizes(ps):
     (4, 1, [256, 257], [256, 600]),
 ])
 def test_prompts(heads, kv_heads, q_lens, kv_lens, dtype, hd):
-    run(len(q_lens) * 7 + heads, q_lens, kv_lens, heads, kv_heads, hd, 16, dtype, tail=5)
+    for width in (0, WIDE):
+        run(len(q_lens) * 7 + heads, q_lens, kv_lens, heads, kv_heads, hd, 16, dtype, tail=5, width=width)
 
 
 @pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1], [40, 90, 300]), ([100, 3, 1], [180, 90, 300]), ([200, 200], [200, 261])])
@@ -93,16 +101,18 @@ def test_scores_and_masks(q_lens, kv_lens, kw):
     kw = dict(kw)
     if "prefix_lens" in kw:
         kw["prefix_lens"] = kw["prefix_lens"][: len(q_lens)]
-    run(31, q_lens, kv_lens, 4, 2, 128, 16, BF, **kw)
-    run(32, q_lens, kv_lens, 6, 2, 64, 32, FP, **kw)
+    for width in (0, WIDE):
+        run(31, q_lens, kv_lens, 4, 2, 128, 16, BF, width=width, **kw)
+        run(32, q_lens, kv_lens, 6, 2, 64, 32, FP, width=width, **kw)
 
 
 def test_rows_and_sequences_that_see_nothing():
     """No keys at all, more new tokens than keys, no new tokens: zeros and -inf where nothing is seen."""
-    run(5, [1, 1, 1], [0, 3, 0], 4, 2, ragged=False)
-    run(6, [3, 0, 5, 1, 0], [0, 9, 2, 0, 0], 4, 2, tail=2)
-    run(7, [200, 0, 3], [140, 50, 0], 4, 2)
-    run(8, [1, 130], [0, 5], 8, 1, prefix=19)
+    for width in (0, WIDE):
+        run(5, [1, 1, 1], [0, 3, 0], 4, 2, ragged=False, width=width)
+        run(6, [3, 0, 5, 1, 0], [0, 9, 2, 0, 0], 4, 2, tail=2, width=width)
+        run(7, [200, 0, 3], [140, 50, 0], 4, 2, width=width)
+        run(8, [1, 130], [0, 5], 8, 1, prefix=19, width=width)
 
 
 def wide_run(q_lens, kv_lens, heads, kv_heads, hd, dtype, ps=16, width=4096, **kw):
@@ -142,10 +152,11 @@ def test_more_sequences_than_a_block_has_threads():
 
 
 @pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [700, 90]), ([300], [700])])
+@pytest.mark.parametrize("width", [0, WIDE])
 @pytest.mark.parametrize("rising", [True, False])
-def test_scores_that_rise_and_fall_along_the_keys(q_lens, kv_lens, rising):
+def test_scores_that_rise_and_fall_along_the_keys(q_lens, kv_lens, rising, width):
     """The running maximum moves in every tile, or never after the first; scores of several hundred, one key wins."""
-    m = ref.make(5, q_lens, kv_lens, 2, 1, 128, 16, BF)
+    m = ref.make(5, q_lens, kv_lens, 2, 1, 128, 16, BF, width=width)
     for b, n in enumerate(kv_lens):
         for j in range(n):
             x = (j if rising else n - j) / n
@@ -184,13 +195,22 @@ def test_long_keys_and_few_sequences():
     run(9, [1], [5003], 4, 2, ragged=False)
     run(10, [2, 1], [3001, 1], 3, 1, hd=64, dtype=FP)
     run(11, [40], [2500], 4, 1)
+    run(12, [3, 1], [10, 9000], 40, 1)
 
 
 @pytest.mark.parametrize("prefix", [1, 16, 100, 333])
-@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1, 1], [1, 9, 70, 33]), ([3, 1, 40], [3, 9, 140]), ([1] * 20, list(range(1, 21))), ([150], [200])])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1, 1], [1, 9, 70, 33]), ([3, 1, 40], [3, 9, 140]), ([1] * 20, list(range(1, 21))), ([150], [200]), ([290, 1], [300, 20])])
 def test_shared_prefix(prefix, q_lens, kv_lens):
-    run(prefix, q_lens, kv_lens, 8, 2, prefix=prefix, tail=1)
-    run(prefix + 1, q_lens, kv_lens, 3, 3, hd=64, ps=32, dtype=FP, prefix=prefix, cap=5.0, slopes=True)
+    for width in (0, WIDE):
+        run(prefix, q_lens, kv_lens, 8, 2, prefix=prefix, tail=1, width=width)
+        run(prefix + 1, q_lens, kv_lens, 3, 3, hd=64, ps=32, dtype=FP, prefix=prefix, cap=5.0, slopes=True, width=width)
+
+
+def test_shared_prefix_long():
+    """A prefix that one row's share of CTAs cuts into ranges, for few rows and for many."""
+    run(71, [1, 1], [5, 40], 8, 2, prefix=5000)
+    run(72, [1, 2], [5, 40], 3, 1, prefix=4100, hd=64, dtype=FP, slopes=True)
+    run(73, [60, 1], [60, 3], 40, 2, prefix=700)
 
 
 def test_shared_prefix_equals_attention_over_the_whole_sequence():
