@@ -644,6 +644,20 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             pages[1] = pages[2];
             pages[2] = i + 3 < n ? page_of(t0 + i + 3) : -1;
         }
+        if (ok && n && see < t1 * PP_KEYS) {
+            // The last tile's rows of V behind the last key that is seen: zeros (their weights are zero, but a page may hold
+            // anything there, and 0 * NaN is NaN).  V of the last tile was asked for last; this warp knows its turn of the
+            // ring (one that had not followed the ring would take the barrier's earlier turns for it).
+            const uint32_t slot = (count - 1) % S::STAGES, valid = see - (t1 - 1) * PP_KEYS;
+            if ((ok = pp_wait(&full[slot], ((count - 1) / S::STAGES) & 1, gave_up))) {
+                for (uint32_t i = valid * 8 + lane; i < PP_KEYS * 8; i += 32)
+#pragma unroll
+                    for (uint32_t p = 0; p < HD / 64; p++) *reinterpret_cast<uint4*>(sR + slot * S::TILE + p * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) pp_arrive(cleaned);
+            }
+        }
         if (!ok)  // given up: let the copies in flight land before the memory goes
             for (uint32_t i = count > S::STAGES ? count - S::STAGES : 0; i < count; i++) pp_land(&full[i % S::STAGES], (i / S::STAGES) & 1);
       } else if (warp == 9 && n) {
@@ -686,7 +700,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 }
                 return got;
             };
-            // the last tile of V: the rows behind the last key that is seen are zeroed by the next warp
+            // the last tile of V: the loader clears the rows behind the last key that is seen
             auto next_value = [&](uint32_t i, uint32_t& slot) -> bool {
                 if (i + 1 == n && see < (t0 + n) * PP_KEYS && !pp_wait(cleaned, 0, gave_up)) return false;
                 return next(slot);
@@ -737,18 +751,6 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 pp_land(drained, 0);
             }
         }
-      } else if (warp == 10 && n && see < t1 * PP_KEYS) {
-        // ---- the last tile's rows of V behind the last key that is seen: zeros (their weights are zero, but a page may
-        // hold anything there, and 0 * NaN is NaN).  In the order of the loads V of the last tile comes last.
-        const uint32_t at = 2 * n - 1, slot = at % S::STAGES, valid = see - (t1 - 1) * PP_KEYS;
-        if (pp_wait(&full[slot], (at / S::STAGES) & 1, gave_up)) {
-            for (uint32_t i = valid * 8 + lane; i < PP_KEYS * 8; i += 32)
-#pragma unroll
-                for (uint32_t p = 0; p < HD / 64; p++) *reinterpret_cast<uint4*>(sR + slot * S::TILE + p * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        __syncwarp();
-        if (lane == 0) pp_arrive(cleaned);
       }
     }
     pp_before();

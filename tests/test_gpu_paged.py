@@ -115,6 +115,14 @@ def test_rows_and_sequences_that_see_nothing():
         run(8, [1, 130], [0, 5], 8, 1, prefix=19, width=width)
 
 
+@pytest.mark.parametrize("hd,dtype", [(64, FP), (128, BF)])
+def test_prompts_of_many_tiles_in_one_block(hd, dtype):
+    """Enough blocks for every SM, so that one takes all its keys: the ring of tiles goes round several times, and the last
+    tile's unused rows (NaN here) are cleared in the right turn of it."""
+    run(3, [260] * 5, [900, 1000, 1111, 260, 1290], 8, 8, hd, 16, dtype, width=WIDE)
+    run(4, [130] * 10, [600 + 37 * i for i in range(10)], 8, 8, hd, 64, dtype, width=WIDE, cap=9.0)
+
+
 def wide_run(q_lens, kv_lens, heads, kv_heads, hd, dtype, ps=16, width=4096, **kw):
     """As run(), with a table far wider than the sequences need: the lengths' upper bound decides how the work is cut."""
     m = ref.make(77, q_lens, kv_lens, heads, kv_heads, hd, ps, dtype)
