@@ -226,7 +226,7 @@ static PgArgs pg_args(const qb200_paged_kv* kv, const qb200_paged_batch* b, uint
     return a;
 }
 
-static qb200_status pg_sms(uint32_t* n) {
+qb200_status pg_sms(uint32_t* n) {
     static int count[64] = {};
     int dev = 0;
     QB_CUDA_TRY(cudaGetDevice(&dev));

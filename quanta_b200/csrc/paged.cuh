@@ -208,6 +208,7 @@ __device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_
     pg_store4<T, HD>(a, pg_end(a, token, head, m, l, col == 0), col, v);
 }
 
+qb200_status pg_sms(uint32_t* n);  // SMs of the current device
 // Attention for few rows (paged_rows.cu): how it runs and the floats of partial results that takes.
 struct PgRows {
     bool units;      // a cluster of 2^c_log CTAs per unit of 16 rows, row_tiles of them a sequence and K/V head; otherwise equal runs of all tiles, and a second kernel

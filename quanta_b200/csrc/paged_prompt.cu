@@ -2,7 +2,7 @@
 // bounded by the tensor pipe and, as closely, by the exponentials (128 x 128 scores cost 1024 cycles of either at head
 // dim 128: 4096 multiply-adds and 16 exponentials a cycle and SM).
 //
-// A unit is 256 packed rows of a sequence and one K/V head, over one of `splits` ranges of its keys; one CTA each, the
+// A unit is 256 (or 128) packed rows of a sequence and one K/V head, over one of `splits` ranges of its keys; one CTA each, the
 // longest first (12 prompts of mixed lengths: 312 us with the sequences in the order of the batch, 262 like this, 52 of them other kernels).  The rows are two tiles of 128 whose steps alternate on the tensor pipe, so that one tile's products
 // run under the other's softmax.  Per step of 128 keys and tile: S = Q K^T (tcgen05.mma, both operands in shared
 // memory, accumulator in TMEM), a warpgroup turns S into P (a thread owns a row, so the row's maximum and sum need no
@@ -27,7 +27,7 @@ namespace qb {
 // scores a thread, take 216, the third one keeps 72.
 constexpr uint32_t PP_THREADS = 384, PP_MORE = 216, PP_LESS = 72;
 static_assert(2 * PP_MORE + PP_LESS == 3 * 168, "the shares add up to what the launch gets");
-constexpr uint32_t PP_KEYS = 128, PP_ROWS = 128, PP_BLOCK = 256;
+constexpr uint32_t PP_KEYS = 128, PP_ROWS = 128;
 constexpr uint32_t PP_POLLS = 1u << 22;
 template <uint32_t HD> struct PpShape {
     static constexpr uint32_t PANEL = 128 * 128;            // 128 rows of 64 elements
@@ -168,14 +168,14 @@ __device__ __forceinline__ uint64_t pp_pair(float lo, float hi) {
 
 struct PpArgs {
     PgArgs g;
-    uint32_t splits, min_rows;
+    uint32_t splits, min_rows, block;  // block: rows of a unit, 256 or 128
     float* parts_acc;  // [splits][tokens * heads][hd] and [splits][tokens * heads][2], splits > 1
     float* parts_ml;
 };
 
 __device__ __forceinline__ uint32_t pp_blocks(const PpArgs& a, const PgSeq& s) {
     const uint32_t rows = s.q_len * a.g.group;
-    return rows < a.min_rows ? 0 : (rows + PP_BLOCK - 1) / PP_BLOCK;
+    return rows < a.min_rows ? 0 : (rows + a.block - 1) / a.block;
 }
 
 template <typename T, uint32_t HD, bool SCORED>
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     const uint32_t b = s_seq, block = s_before - 1 - want;
     const uint32_t kvh = blockIdx.x / pa.splits % a.kv_heads, split = blockIdx.x % pa.splits;
     const PgSeq sq = s_found;
-    const uint32_t all_rows = sq.q_len * a.group, row0 = block * PP_BLOCK, rows = min(PP_BLOCK, all_rows - row0);
+    const uint32_t all_rows = sq.q_len * a.group, row0 = block * pa.block, rows = min(pa.block, all_rows - row0);
     const uint32_t see = pg_limit(sq, (row0 + rows - 1) / a.group);  // keys the block's last token sees (the most)
     const uint32_t n_all = (see + PP_KEYS - 1) / PP_KEYS;
     const uint32_t t0 = n_all * split / pa.splits, t1 = n_all * (split + 1) / pa.splits, n = t1 - t0;  // (below 2^24 tiles, at most 148 splits)
@@ -821,17 +821,26 @@ __global__ void __launch_bounds__(128) k_paged_prompt_join(const __grid_constant
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-// Blocks of 256 rows that the call can have, over all sequences.
-static uint64_t pp_most_blocks(const PgArgs& a) {
+// Units that the call can have, over all sequences, with blocks of so many rows.
+static uint64_t pp_most_units(const PgArgs& a, uint32_t block) {
     const uint64_t rows = (uint64_t)a.tokens * a.group;
-    if (a.shared) return div_ceil(rows, PP_BLOCK);
-    if (!a.cu_q) return (uint64_t)a.batch * div_ceil(a.group, PP_BLOCK);
-    return rows / PP_BLOCK + (a.batch < a.tokens ? a.batch : a.tokens);
+    if (a.shared) return div_ceil(rows, block) * a.kv_heads;
+    if (!a.cu_q) return a.batch * div_ceil(a.group, block) * a.kv_heads;
+    return (rows / block + (a.batch < a.tokens ? a.batch : a.tokens)) * a.kv_heads;
+}
+
+static uint64_t pp_most_keys(const PgArgs& a) { return a.shared ? a.shared : (uint64_t)a.width << a.ps_log; }
+
+// Blocks of one tile of rows for short keys, where all of them fit the SMs at once: more SMs work and fewer partial results
+// are joined (us with 128 / 256 rows, 32 / 8 heads: 512 tokens 15.1 / 23.6, 1024 tokens 24.2 / 24.0; 512 tokens against 4000 keys 67 / 51:
+// a tile of keys then serves half the rows).
+static uint32_t pp_block(const PgArgs& a, uint32_t sms) {
+    return pp_most_units(a, PP_ROWS) <= sms && pp_most_keys(a) <= 6 * PP_KEYS ? PP_ROWS : 2 * PP_ROWS;
 }
 
 uint32_t pg_prompt_splits(const PgArgs& a, uint32_t sms) {
     // fewer units than SMs: every unit's keys are cut so that all SMs have work, into ranges of at least two tiles
-    const uint64_t units = pp_most_blocks(a) * a.kv_heads, keys = a.shared ? a.shared : (uint64_t)a.width << a.ps_log;
+    const uint64_t units = pp_most_units(a, pp_block(a, sms)), keys = pp_most_keys(a);
     const uint64_t by_keys = div_ceil(keys, 2 * PP_KEYS), by_sms = units ? sms / units : 1, s = by_keys < by_sms ? by_keys : by_sms;
     return s > 1 ? (uint32_t)s : 1;
 }
@@ -891,7 +900,11 @@ qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t 
     pa.min_rows = min_rows;
     pa.parts_acc = a.parts;
     pa.parts_ml = a.parts + (uint64_t)splits * a.tokens * a.group * a.kv_heads * hd;
-    const uint64_t units = pp_most_blocks(a) * a.kv_heads * splits;
+    uint32_t sms = 0;
+    const qb200_status got = pg_sms(&sms);
+    if (got) return got;
+    pa.block = pp_block(a, sms);
+    const uint64_t units = pp_most_units(a, pa.block) * splits;
     if (units > 0x7FFFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, "paged attention: 2^31 blocks of rows or more");
     const uint32_t grid = (uint32_t)units;
     // a score that is not a positive multiple of q . k takes the general form (the plain one keeps its maximum in q . k)

@@ -160,7 +160,7 @@ def paged_rope_append(batch: PagedBatch, q: Optional[torch.Tensor], k: torch.Ten
     if q is None:
         _want(q_out is None, "paged_rope_append: q_out without q")
     elif q_out is None:
-        q_out = cache.k.new_empty((tokens, heads * cache.head_dim))
+        q_out = cache.k.new_empty(tokens, heads * cache.head_dim)
     else:
         _want(q_out.shape == q.shape and q_out.dtype == cache.dtype and q_out.device == dev and q_out.is_contiguous(),
               "paged_rope_append: q_out must be contiguous, of q's shape and the cache's type")
@@ -177,7 +177,7 @@ def _attend(who: str, batch: PagedBatch, q: torch.Tensor, slopes, out, lse):
     if q.dtype != cache.dtype:
         _bad(f"{who}: q is {q.dtype}, the cache {cache.dtype}", L.ERR_NOT_SUPPORTED)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != cache.dtype or out.device != dev or not out.is_contiguous():
         _bad(f"{who}: out must be contiguous, of q's shape and the cache's type")
     if lse is not None and (lse.shape != (tokens, heads) or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous()):
