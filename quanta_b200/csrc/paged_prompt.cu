@@ -144,21 +144,19 @@ __device__ __forceinline__ uint64_t pp_pack2(float x) {
 __device__ __forceinline__ void pp_mul2(float& x0, float& x1, uint64_t m2) {
     asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tmul.rn.f32x2 t, t, %2;\n\tmov.b64 {%0, %1}, t;\n\t}" : "+f"(x0), "+f"(x1) : "l"(m2));
 }
-// tanh of a pair with |x| <= 1/2: x (1 + u P(u)), u = x^2, P the cubic that is best there (absolute error 4.3e-9, fitted
-// by reweighted least squares), on the multiply-add pipe: six instructions a pair, where the exponential and the
-// reciprocal of the general form would triple the load of the pipe that already bounds the softmax.  (The caller scales x:
-// with coefficients multiplied by b^9, b^7, b^5, b^3 and b it is tanh(b x) for |b x| <= 1/2.)
-__device__ __forceinline__ void pp_tanh2(float& x0, float& x1, uint64_t c3, uint64_t c2, uint64_t c1, uint64_t c0, uint64_t one) {
+// tanh(b x) of a pair with |b x| <= 0.3: x (b + u (k0 + k1 u)), u = x^2, with b^3 and b^5 in the coefficients of the
+// polynomial that is best there (absolute error 2.9e-7, fitted by reweighted least squares), on the multiply-add pipe: four
+// instructions a pair, where the exponential and the reciprocal of the general form would triple the load of the pipe that
+// already bounds the softmax.
+__device__ __forceinline__ void pp_tanh2(float& x0, float& x1, uint64_t k1, uint64_t k0, uint64_t b) {
     asm("{\n\t.reg .b64 x, u, p;\n\t"
         "mov.b64 x, {%0, %1};\n\t"
         "mul.rn.f32x2 u, x, x;\n\t"
         "fma.rn.f32x2 p, u, %2, %3;\n\t"
         "fma.rn.f32x2 p, p, u, %4;\n\t"
-        "fma.rn.f32x2 p, p, u, %5;\n\t"
-        "fma.rn.f32x2 p, p, u, %6;\n\t"
         "mul.rn.f32x2 x, x, p;\n\t"
         "mov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(x0), "+f"(x1) : "l"(c3), "l"(c2), "l"(c1), "l"(c0), "l"(one));
+        : "+f"(x0), "+f"(x1) : "l"(k1), "l"(k0), "l"(b));
 }
 __device__ __forceinline__ uint64_t pp_pair(float lo, float hi) {
     uint64_t r;
@@ -375,16 +373,13 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
 #pragma unroll
                         for (uint32_t k = 0; k < 4; k++) far[k] = fmaxf(fmaxf(far[k], fabsf(s[i + k])), fabsf(s[i + 4 + k]));
                     const float b = a.score_mul;
-                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * fabsf(b) <= 0.5f && fabsf(b) <= 64.0f))) {  // (b^9 stays in range)
+                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * fabsf(b) <= 0.3f && fabsf(b) <= 64.0f))) {  // (b^5 stays in range)
 #pragma unroll
                         for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i] * b, 1.0f);
                     } else {
-                        // tanh(b s) with b in the coefficients
-                        const float b2 = b * b;
-                        const uint64_t k3 = pp_pack2(0.017005980014801025f * b2 * b2 * b2 * b2 * b), k2 = pp_pack2(-0.05292436107993126f * b2 * b2 * b2 * b),
-                                       k1 = pp_pack2(0.13323938846588135f * b2 * b2 * b), k0 = pp_pack2(-0.33333051204681396f * b2 * b), one = pp_pack2(b);
+                        const uint64_t k1 = pp_pack2(0.12640675902366638f * b * b * b * b * b), k0 = pp_pack2(-0.33312109112739563f * b * b * b), k = pp_pack2(b);
 #pragma unroll
-                        for (uint32_t i = 0; i < 128; i += 2) pp_tanh2(s[i], s[i + 1], k3, k2, k1, k0, one);
+                        for (uint32_t i = 0; i < 128; i += 2) pp_tanh2(s[i], s[i + 1], k1, k0, k);
                     }
                 }
                 if (a.slopes) {
