@@ -158,11 +158,22 @@ __device__ __forceinline__ void pp_tanh2(float& x0, float& x1, uint64_t k1, uint
         "mov.b64 {%0, %1}, x;\n\t}"
         : "+f"(x0), "+f"(x1) : "l"(k1), "l"(k0), "l"(b));
 }
-__device__ __forceinline__ uint64_t pp_pair(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
+// The numbers 0 .. 127 as pairs of floats.
+__constant__ uint64_t pp_index[64] = {
+    0x3F80000000000000ull, 0x4040000040000000ull, 0x40A0000040800000ull, 0x40E0000040C00000ull, 0x4110000041000000ull,
+    0x4130000041200000ull, 0x4150000041400000ull, 0x4170000041600000ull, 0x4188000041800000ull, 0x4198000041900000ull,
+    0x41A8000041A00000ull, 0x41B8000041B00000ull, 0x41C8000041C00000ull, 0x41D8000041D00000ull, 0x41E8000041E00000ull,
+    0x41F8000041F00000ull, 0x4204000042000000ull, 0x420C000042080000ull, 0x4214000042100000ull, 0x421C000042180000ull,
+    0x4224000042200000ull, 0x422C000042280000ull, 0x4234000042300000ull, 0x423C000042380000ull, 0x4244000042400000ull,
+    0x424C000042480000ull, 0x4254000042500000ull, 0x425C000042580000ull, 0x4264000042600000ull, 0x426C000042680000ull,
+    0x4274000042700000ull, 0x427C000042780000ull, 0x4282000042800000ull, 0x4286000042840000ull, 0x428A000042880000ull,
+    0x428E0000428C0000ull, 0x4292000042900000ull, 0x4296000042940000ull, 0x429A000042980000ull, 0x429E0000429C0000ull,
+    0x42A2000042A00000ull, 0x42A6000042A40000ull, 0x42AA000042A80000ull, 0x42AE000042AC0000ull, 0x42B2000042B00000ull,
+    0x42B6000042B40000ull, 0x42BA000042B80000ull, 0x42BE000042BC0000ull, 0x42C2000042C00000ull, 0x42C6000042C40000ull,
+    0x42CA000042C80000ull, 0x42CE000042CC0000ull, 0x42D2000042D00000ull, 0x42D6000042D40000ull, 0x42DA000042D80000ull,
+    0x42DE000042DC0000ull, 0x42E2000042E00000ull, 0x42E6000042E40000ull, 0x42EA000042E80000ull, 0x42EE000042EC0000ull,
+    0x42F2000042F00000ull, 0x42F6000042F40000ull, 0x42FA000042F80000ull, 0x42FE000042FC0000ull,
+};
 
 struct PpArgs {
     PgArgs g;
@@ -340,14 +351,17 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         float slope = 0.0f;
         int32_t pos = 0;
         if (SCORED && a.slopes) {
-            slope = a.slopes[head] * PG_LOG2E;
+            slope = a.slopes[head];
             pos = pg_position(a, sq, token);
         }
         const uint32_t t_lane = tmem + (((warp & 3) * 32) << 16);
         const uint32_t t_s = t_lane + w * S::S_COLS, t_o = t_lane + S::O_COL + w * 128;
         // the factor that the exponential still has to apply: cap, or the whole scale of the plain form
-        const float c = !SCORED ? a.score_mul : a.slopes || a.cap_mul == 0.0f ? 1.0f : a.cap_mul;
+        // (a scale that is not positive is applied before)
+        const bool before = SCORED && a.cap_mul == 0.0f && !(a.score_mul > 1e-30f);
+        const float c = SCORED && a.cap_mul != 0.0f ? a.cap_mul : before ? 1.0f : a.score_mul;
         const uint64_t c2 = pp_pack2(c);
+        if (SCORED) slope *= PG_LOG2E / c;  // in units of what the exponential scales
         const float slack = 8.0f / c;  // 2^8 in units of the score (c is positive)
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         bool ok = true;
@@ -360,8 +374,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             for (uint32_t i = 0; i < 4; i++) pp_tmem_ld32(t_s + i * 32, s + i * 32);
             pp_ld_done();
             const uint32_t key0 = t * PP_KEYS;
+            float shift = 0.0f;  // of all the row's scores of this tile
             if (SCORED) {
-                if (a.cap_mul == 0.0f && !a.slopes) {
+                if (before) {
                     const uint64_t mul2 = pp_pack2(a.score_mul);
 #pragma unroll
                     for (uint32_t i = 0; i < 128; i += 2) pp_mul2(s[i], s[i + 1], mul2);
@@ -383,27 +398,19 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     }
                 }
                 if (a.slopes) {
-                    const uint64_t up2 = pp_pack2(a.cap_mul != 0.0f ? a.cap_mul : a.score_mul);
                     const int32_t d = pos - (int32_t)key0;
-                    if (__all_sync(0xFFFFFFFFu, d >= (int32_t)PP_KEYS - 1)) {  // no key behind the row's own place: linear in the key
-                        uint64_t off[4];
-                        const float df = (float)d;
+                    if (__all_sync(0xFFFFFFFFu, d >= (int32_t)PP_KEYS - 1)) {
+                        // no key behind the row's own place: slope * (i - d) for key i, its constant part left to the reference
+                        shift = -slope * (float)d;
+                        const uint64_t slope2 = pp_pack2(slope);
 #pragma unroll
-                        for (uint32_t k = 0; k < 4; k++) off[k] = pp_pair(slope * (float)(2 * k), slope * (float)(2 * k + 1));
-#pragma unroll
-                        for (uint32_t i = 0; i < 128; i += 8) {
-                            const float at = slope * ((float)i - df);
-#pragma unroll
-                            for (uint32_t k = 0; k < 4; k++) {
-                                asm("{\n\t.reg .b64 t, x;\n\tmov.b64 t, {%2, %2};\n\tadd.rn.f32x2 t, t, %3;\n\tmov.b64 x, {%0, %1};\n\t"
-                                    "fma.rn.f32x2 x, x, %4, t;\n\tmov.b64 {%0, %1}, x;\n\t}"
-                                    : "+f"(s[i + 2 * k]), "+f"(s[i + 2 * k + 1]) : "f"(at), "l"(off[k]), "l"(up2));
-                            }
-                        }
+                        for (uint32_t i = 0; i < 128; i += 2)
+                            asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tfma.rn.f32x2 t, %2, %3, t;\n\tmov.b64 {%0, %1}, t;\n\t}"
+                                : "+f"(s[i]), "+f"(s[i + 1]) : "l"(slope2), "l"(pp_index[i >> 1]));
                     } else {
-                        const float up = a.cap_mul != 0.0f ? a.cap_mul : a.score_mul, d0 = (float)d;
+                        const float d0 = (float)d;
 #pragma unroll
-                        for (uint32_t i = 0; i < 128; i++) s[i] = fmaf(-slope, fabsf(d0 - (float)i), s[i] * up);
+                        for (uint32_t i = 0; i < 128; i++) s[i] = fmaf(-slope, fabsf(d0 - (float)i), s[i]);
                     }
                 }
             }
@@ -419,7 +426,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 for (uint32_t k = 0; k < 4; k++) mx[k] = fmaxf(fmaxf(mx[k], s[i + k]), s[i + 4 + k]);  // one three-way maximum
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], s[124 + k]);
-            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) + shift;
             if (__any_sync(0xFFFFFFFFu, mt > m + slack)) {
                 const float mn = fmaxf(m, mt);
                 const float f = m == -INFINITY ? 0.0f : pg_exp2((m - mn) * c);
@@ -439,7 +446,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     pp_st_done();
                 }
             }
-            const uint64_t mc2 = pp_pack2(m == -INFINITY ? 0.0f : -m * c);
+            const uint64_t mc2 = pp_pack2(m == -INFINITY ? 0.0f : (shift - m) * c);
             uint32_t pk[32];
 #pragma unroll
             for (uint32_t h = 0; h < 2; h++) {
