@@ -84,6 +84,11 @@ __device__ __forceinline__ void pp_load(uint32_t dst, const CUtensorMap* map, in
         "r"(x), "r"(y), "r"(z), "r"(w), "r"(pp_smem(bar))
         : "memory");
 }
+__device__ __forceinline__ void pp_load3(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
+                 "r"(y), "r"(z), "r"(pp_smem(bar))
+                 : "memory");
+}
 // Shared-memory matrix descriptors, 128-byte swizzle.  K-major (Q, K): 8-row groups 1024 bytes apart.  MN-major (V as
 // [keys][columns]): groups of 8 keys 1024 bytes apart, panels of 64 columns 16 KB apart.
 __device__ __forceinline__ uint64_t pp_desc(uint32_t saddr, uint32_t lead) {
@@ -178,6 +183,7 @@ __constant__ uint64_t pp_index[64] = {
 struct PpArgs {
     PgArgs g;
     uint32_t splits, min_rows, block;  // block: rows of a unit, 256 or 128
+    uint32_t q_boxes;  // Q by TMA: 128 rows are a box of whole tokens
     float* parts_acc;  // [splits][tokens * heads][hd] and [splits][tokens * heads][2], splits > 1
     float* parts_ml;
 };
@@ -189,7 +195,7 @@ __device__ __forceinline__ uint32_t pp_blocks(const PpArgs& a, const PgSeq& s) {
 
 template <typename T, uint32_t HD, bool SCORED>
 __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                                                                const __grid_constant__ PpArgs pa) {
+                                                                const __grid_constant__ CUtensorMap qmap, const __grid_constant__ PpArgs pa) {
     using S = PpShape<HD>;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -216,7 +222,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             pp_init(&full[i], 1);
             pp_init(&empty[i], 1);
         }
-        pp_init(q_full, 8);
+        pp_init(q_full, pa.q_boxes ? 1 : 8);
         pp_init(cleaned, 1);
         pp_init(drained, 1);
         for (uint32_t i = 0; i < 2; i++) {
@@ -308,8 +314,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     const uint32_t t0 = n_all * split / pa.splits, t1 = n_all * (split + 1) / pa.splits, n = t1 - t0;  // (below 2^24 tiles, at most 148 splits)
     const bool dual = rows <= PP_ROWS;
 
-    // ---- Q to shared memory (all of it in flight at once; rows past the last one are zeros) ----
-    if (warp < 8 && (!dual || warp < 4)) {
+    // ---- Q to shared memory.  Where the group divides 128 the loader asks for whole boxes; otherwise row by row, all of it in
+    // flight at once, and rows past the last one are zeros (1500 cycles of a unit more) ----
+    if (!pa.q_boxes && warp < 8 && (!dual || warp < 4)) {
         constexpr uint32_t CH = HD / 8, STEP = 128 / CH;
         const uint32_t w = warp >> 2, wt = tid & 127, ch = wt % CH, first = w * PP_ROWS, t_rows = min(PP_ROWS, rows - first);
         const uint32_t whole = STEP / a.group, rest = STEP % a.group;
@@ -339,10 +346,12 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         const uint32_t w = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t first = dual ? 0 : w * PP_ROWS;  // the tile's first row of the block
         const uint32_t t_rows = min(PP_ROWS, rows - first);
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) pp_arrive(q_full);
+        if (!pa.q_boxes) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) pp_arrive(q_full);
+        }
 
         const uint32_t my = min(r, t_rows - 1);  // a row past the last one runs along with it and is not stored
         const uint32_t row = row0 + first + my, token = row / a.group, head = kvh * a.group + row % a.group;
@@ -634,6 +643,18 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             count++;
             if (++st == S::STAGES) st = 0;
         };
+        if (pa.q_boxes && lane == 0) {
+            // (rows behind the sequence's last one are the next sequence's, or zeros: their results are not stored)
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the search used this memory
+            const uint32_t tiles = dual ? 1 : 2;
+            pp_expect(q_full, tiles * S::TILE);
+            for (uint32_t w = 0; w < tiles; w++)
+#pragma unroll
+                for (uint32_t p = 0; p < HD / 64; p++)
+                    pp_load3(pp_smem(sQ) + w * S::TILE + p * S::PANEL, &qmap, (int32_t)(p * 64), (int32_t)(kvh * a.group),
+                             (int32_t)(sq.q0 + (row0 + w * PP_ROWS) / a.group), q_full);
+        }
+        __syncwarp();
         int32_t pages[3];  // of tiles t, t + 1, t + 2
 #pragma unroll
         for (uint32_t i = 0; i < 3; i++) pages[i] = i < n ? page_of(t0 + i) : -1;
@@ -866,7 +887,7 @@ static PpEncodeFn pp_encode_fn() {
 }
 
 template <typename T, uint32_t HD, bool SCORED>
-static qb200_status launch_prompt(const PpArgs& pa, uint32_t grid, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
+static qb200_status launch_prompt(const PpArgs& pa, uint32_t grid, const CUtensorMap (&map)[3], cudaStream_t st) {
     static bool attr_set[64] = {};
     int dev = 0;
     QB_CUDA_TRY(cudaGetDevice(&dev));
@@ -874,7 +895,7 @@ static qb200_status launch_prompt(const PpArgs& pa, uint32_t grid, const CUtenso
         QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_prompt<T, HD, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PpShape<HD>::SMEM));
         attr_set[dev & 63] = true;
     }
-    QB_CUDA_TRY(pg_launch(k_paged_prompt<T, HD, SCORED>, dim3(grid), dim3(PP_THREADS), PpShape<HD>::SMEM, st, kmap, vmap, pa));
+    QB_CUDA_TRY(pg_launch(k_paged_prompt<T, HD, SCORED>, dim3(grid), dim3(PP_THREADS), PpShape<HD>::SMEM, st, map[0], map[1], map[2], pa));
     if (pa.splits > 1) {
         const uint64_t rows = (uint64_t)pa.g.tokens * pa.g.group * pa.g.kv_heads, per = 128 / (HD / 4);
         QB_CUDA_TRY(pg_launch(k_paged_prompt_join<T, HD>, dim3((uint32_t)((rows + per - 1) / per)), dim3(128), 0, st, pa));
@@ -886,7 +907,7 @@ qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t 
     PpEncodeFn enc = pp_encode_fn();
     if (!enc) return fail(QB200_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled is not available from this driver");
     const uint32_t ps = 1u << a.ps_log;
-    CUtensorMap map[2];
+    CUtensorMap map[3];
     for (int i = 0; i < 2; i++) {
         const cuuint64_t dims[4] = {hd, ps, a.kv_heads, a.n_pages};
         const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)ps * hd * 2, (cuuint64_t)a.kv_heads * ps * hd * 2};
@@ -898,6 +919,17 @@ qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t 
     }
     PpArgs pa = {};
     pa.g = a;
+    map[2] = map[0];  // a valid map either way; unused without boxes
+    if (PP_ROWS % a.group == 0) {
+        // Q as [tokens][heads][hd]: 128 packed rows are 128 / group tokens of a group's heads
+        pa.q_boxes = 1;
+        const cuuint64_t dims[3] = {hd, (cuuint64_t)a.group * a.kv_heads, a.tokens}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)a.q_stride * 2};
+        const cuuint32_t box[3] = {64, a.group, PP_ROWS / a.group}, estr[3] = {1, 1, 1};
+        const CUresult cr = enc(&map[2], dtype == QB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(a.q),
+                                dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (cr != CUDA_SUCCESS) return fail(QB200_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled (Q) failed with code " + std::to_string((int)cr));
+    }
     pa.splits = splits;
     pa.min_rows = min_rows;
     pa.parts_acc = a.parts;
@@ -912,11 +944,11 @@ qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t 
     // a score that is not a positive multiple of q . k takes the general form (the plain one keeps its maximum in q . k)
     const bool scored = a.cap_mul != 0.0f || a.slopes || !(a.score_mul > 1e-30f);
     if (dtype == QB200_BF16) {
-        if (hd == 128) return scored ? launch_prompt<__nv_bfloat16, 128, true>(pa, grid, map[0], map[1], st) : launch_prompt<__nv_bfloat16, 128, false>(pa, grid, map[0], map[1], st);
-        return scored ? launch_prompt<__nv_bfloat16, 64, true>(pa, grid, map[0], map[1], st) : launch_prompt<__nv_bfloat16, 64, false>(pa, grid, map[0], map[1], st);
+        if (hd == 128) return scored ? launch_prompt<__nv_bfloat16, 128, true>(pa, grid, map, st) : launch_prompt<__nv_bfloat16, 128, false>(pa, grid, map, st);
+        return scored ? launch_prompt<__nv_bfloat16, 64, true>(pa, grid, map, st) : launch_prompt<__nv_bfloat16, 64, false>(pa, grid, map, st);
     }
-    if (hd == 128) return scored ? launch_prompt<__half, 128, true>(pa, grid, map[0], map[1], st) : launch_prompt<__half, 128, false>(pa, grid, map[0], map[1], st);
-    return scored ? launch_prompt<__half, 64, true>(pa, grid, map[0], map[1], st) : launch_prompt<__half, 64, false>(pa, grid, map[0], map[1], st);
+    if (hd == 128) return scored ? launch_prompt<__half, 128, true>(pa, grid, map, st) : launch_prompt<__half, 128, false>(pa, grid, map, st);
+    return scored ? launch_prompt<__half, 64, true>(pa, grid, map, st) : launch_prompt<__half, 64, false>(pa, grid, map, st);
 }
 
 }  // namespace qb

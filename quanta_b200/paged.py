@@ -124,7 +124,7 @@ def _rows(x: torch.Tensor, heads: int, cache: PagedKVCache, what: str) -> Tuple[
         step, col = x.stride()
         n = width // cache.head_dim
         if n and n * cache.head_dim == width and (n == heads or heads == 0) and col == 1 and x.get_device() == cache._index:
-            return tokens, n, step if tokens > 1 else max(width, step)
+            return tokens, n, step if tokens > 1 else width  # (one row has no next one)
     if x.device != cache.device:
         _bad(f"{what} is on {x.device}, the cache on {cache.device}")
     _bad(f"{what} must be [tokens, {heads or 'heads'} * {cache.head_dim}] with contiguous columns, got {list(shape)}", L.ERR_LENGTH)

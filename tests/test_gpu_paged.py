@@ -307,6 +307,9 @@ def test_strided_queries():
     wide[:, 136: 136 + heads * hd] = m["q"].to(DEV)
     got = paged.paged_attention(batch, wide[:, 136: 136 + heads * hd])
     assert torch.equal(got, paged.paged_attention(batch, m["q"].to(DEV)))
+    one = paged.PagedBatch(cache, batch.table[:1], batch.kv_lens[:1])
+    odd = torch.randn(1, heads * hd + 1, device=DEV).to(BF)[:, : heads * hd]  # a single row, whatever its stride
+    assert torch.equal(paged.paged_attention(one, odd), paged.paged_attention(one, odd.contiguous()))
     # a table that is a window of a wider one
     t = torch.full((3, 40), -1, dtype=torch.int32, device=DEV)
     t[:, 4: 4 + m["table"].shape[1]] = m["table"].to(DEV)
