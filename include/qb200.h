@@ -275,7 +275,8 @@ QB200_API qb200_status qb200_sum_arrays(const float* parts, uint32_t count, uint
  *   positions[t] of cos / sin [n_pos, rot_dim / 2] f32 (NULL: the row's place in its sequence); f32 arithmetic, one
  *   rounding.  q -> q_out [tokens, heads * head_dim] of the cache's type, k and v -> the sequence's pages.  q and
  *   q_out NULL with heads = 0: keys and values alone.  A token whose place would be negative (more new tokens than
- *   keys) is not written.  Two tokens of one call must not have the same place.
+ *   keys) is not written.  Two tokens of one call must not have the same place, and q_out must not
+ *   overlap the inputs.
  * qb200_paged_attention: token at place p of its sequence sees keys 0 .. p (causal), the first prefix_lens[b] keys
  *   too where prefix_lens is given, or all kv_lens[b] keys (causal = 0).  Score = scale * (q . k); softcap (0, or at least 1e-6) > 0: softcap *
  *   tanh(score / softcap); slopes [heads] given: minus slopes[h] * |distance|.  heads is a multiple of kv_heads, head h

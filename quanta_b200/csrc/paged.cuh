@@ -52,8 +52,8 @@ struct PgArgs {
 };
 
 struct PgSeq {
-    uint32_t q0, q_len, kv, see;  // rows [q0, q0 + q_len) of the batch; keys [0, kv); some row sees keys [0, see)
-    uint32_t prefix;
+    uint32_t q0, q_len, kv;  // rows [q0, q0 + q_len) of the batch; keys [0, kv)
+    uint32_t prefix;         // keys that every row sees
 };
 
 __device__ __forceinline__ void pg_report(int32_t* status, int32_t code) { atomicCAS(status, 0, code); }
@@ -65,7 +65,7 @@ __device__ __forceinline__ PgSeq pg_seq(const PgArgs& a, uint32_t b) {
         int32_t n = a.cu_q ? a.cu_q[a.batch] : (int32_t)a.tokens;
         s.q0 = 0;
         s.q_len = n < 0 ? 0u : min((uint32_t)n, a.tokens);
-        s.kv = s.see = a.shared;
+        s.kv = a.shared;
         s.prefix = a.shared;
         return s;
     }
@@ -83,7 +83,7 @@ __device__ __forceinline__ PgSeq pg_seq(const PgArgs& a, uint32_t b) {
     }
     s.q0 = (uint32_t)lo;
     s.q_len = (uint32_t)(hi - lo);
-    s.kv = s.see = (uint32_t)kv;
+    s.kv = (uint32_t)kv;
     const int32_t p = a.prefix_lens ? a.prefix_lens[b] : 0;
     s.prefix = a.causal ? (uint32_t)max(p, 0) : 0xFFFFFFFFu;
     return s;

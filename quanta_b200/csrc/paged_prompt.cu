@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 s_found = mine;
             }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // Q's copies may land on s_kv next
         __syncthreads();
     } else {
         uint32_t* s_sum = reinterpret_cast<uint32_t*>(s_kv);
@@ -296,6 +297,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 s_before = excl + n;
                 s_found = mine;
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncthreads();
             if (s_seq != 0xFFFFFFFFu) break;
         }
@@ -645,7 +647,6 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         };
         if (pa.q_boxes && lane == 0) {
             // (rows behind the sequence's last one are the next sequence's, or zeros: their results are not stored)
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the search used this memory
             const uint32_t tiles = dual ? 1 : 2;
             pp_expect(q_full, tiles * S::TILE);
             for (uint32_t w = 0; w < tiles; w++)
