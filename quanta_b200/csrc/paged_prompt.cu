@@ -808,14 +808,16 @@ __global__ void __launch_bounds__(128) k_paged_prompt_join(const __grid_constant
     }
     float M = -INFINITY, L = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr uint32_t U = 6;  // ranges in flight
+    constexpr uint32_t U = 10;  // ranges in flight
 #pragma unroll 1
     for (uint32_t i0 = 0; i0 < pa.splits; i0 += U) {
         float2 ml[U];
         float4 e[U];
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) {
-            const uint64_t i = min(i0 + u, pa.splits - 1);
+            const uint64_t i = i0 + u;
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            if (i0 + u >= pa.splits) continue;
             ml[u] = *reinterpret_cast<const float2*>(pa.parts_ml + (i * all + row) * 2);
             e[u] = *reinterpret_cast<const float4*>(pa.parts_acc + (i * all + row) * HD + col);
         }
@@ -831,8 +833,8 @@ __global__ void __launch_bounds__(128) k_paged_prompt_join(const __grid_constant
         v.w *= f;
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) {
-            const float g = i0 + u < pa.splits ? pg_weight(ml[u].x, M) : 0.0f;
-            if (g == 0.0f) continue;  // no key there (or a weight below the smallest number)
+            const float g = pg_weight(ml[u].x, M);
+            if (g == 0.0f) continue;  // no range or no key there (or a weight below the smallest number)
             L = fmaf(ml[u].y, g, L);
             v.x = fmaf(e[u].x, g, v.x);
             v.y = fmaf(e[u].y, g, v.y);

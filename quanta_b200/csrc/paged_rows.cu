@@ -152,15 +152,20 @@ struct PrAt {
 };
 __device__ __forceinline__ PgSeq pr_seq(const PgArgs& a, const PgSeq* kept, uint32_t b) { return b < PR_KEPT ? kept[b] : pg_seq(a, b); }
 // n tiles further (not past the unit's end).
-__device__ __forceinline__ void pr_advance(const PgArgs& a, const PgSeq* kept, PrAt& p, uint32_t n) {
+__device__ __forceinline__ void pr_advance(const PgArgs& a, const PgSeq* kept, uint32_t seqs, PrAt& p, uint32_t n) {
     p.left -= n;
     p.t += n;
     if (p.left == 0 || p.t < p.tiles) return;
     p.t = 0;
     if (++p.kvh < a.kv_heads) return;
     p.kvh = 0;
-    do p.s = pr_seq(a, kept, ++p.b);  // (the run goes on, so there is one)
-    while (pr_weight(a, p.s) == 0);
+    do {  // the run goes on, so there is one (but for lengths that another stream changes meanwhile)
+        if (++p.b >= seqs) {
+            p.left = 0;
+            return;
+        }
+        p.s = pr_seq(a, kept, p.b);
+    } while (pr_weight(a, p.s) == 0);
     p.tiles = pr_tiles(p.s);
 }
 
@@ -366,7 +371,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
     int32_t* meta = a.meta + blockIdx.x * 8;
     if (tid == 0) meta[0] = -1;
     PrRun run;
-    if (!pr_find_run(a, a.shared ? 1 : a.batch, kept, run)) return;
+    const uint32_t seqs = a.shared ? 1 : a.batch;
+    if (!pr_find_run(a, seqs, kept, run)) return;
     const uint32_t ring_s = pr_smem(smem + warp * S::WARP), q_s = pr_smem(smem + S::Q);
     float* j_acc = reinterpret_cast<float*>(smem + S::JOIN);
     float* j_ml = reinterpret_cast<float*>(smem + S::ML);
@@ -392,7 +398,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
         n_valid = n_key < ahead.s.kv ? min(ahead.s.kv - n_key, PR_KEYS) : 0;
         n_kvh = ahead.kvh;
         if (n_valid) n_page = a.table[(a.shared ? 0 : (uint64_t)ahead.b * a.table_stride) + (n_key >> a.ps_log)];
-        pr_advance(a, kept, ahead, 1);
+        pr_advance(a, kept, seqs, ahead, 1);
     };
     auto fetch = [&](uint32_t st) {
         if (n_there) {
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
 
         // ---- its end: on to the next unit's Q, then the warps' states are joined, PASS rows at a time ----
         const uint32_t first_tile = run.run1 - here.left;
-        pr_advance(a, kept, here, n);
+        pr_advance(a, kept, seqs, here, n);
         const bool more = here.left != 0;
         if (more) bring_q(here);
         pr_end<HD>(u, j_ml + warp * 2 * PR_ROWS);
