@@ -2,9 +2,12 @@
 // bounded by the tensor pipe and, as closely, by the exponentials (128 x 128 scores cost 1024 cycles of either at head
 // dim 128: 4096 multiply-adds and 16 exponentials a cycle and SM).
 //
-// A unit is 256 (or 128) packed rows of a sequence and one K/V head, over one of `splits` ranges of its keys; one CTA each, the
-// longest first (12 prompts of mixed lengths: 312 us with the sequences in the order of the batch, 262 like this, 52 of them other kernels).  The rows are two tiles of 128 whose steps alternate on the tensor pipe, so that one tile's products
-// run under the other's softmax.  Per step of 128 keys and tile: S = Q K^T (tcgen05.mma, both operands in shared
+// A unit is 256 (or 128) packed rows of a sequence and one K/V head, over one of `splits` ranges of its keys; one CTA
+// each, the longest first (12 prompts of mixed lengths among single tokens: 262 us against 312 with the sequences in the
+// order of the batch).  The rows are two tiles of 128 whose steps alternate on the tensor pipe, so that one tile's
+// products run under the other's softmax: a prompt of 8192 tokens, 32 / 8 heads of 128, runs at 1.25 PFLOP/s (0.75 of
+// measured) in short runs and at 1.05 under the power cap.  A tile's chain bounds it (in cycles: maximum 400,
+// exponentials 1350, then P V of the second half and the next Q K^T 1300).  Per step of 128 keys and tile: S = Q K^T (tcgen05.mma, both operands in shared
 // memory, accumulator in TMEM), a warpgroup turns S into P (a thread owns a row, so the row's maximum and sum need no
 // exchange), P goes back to TMEM over S in the cache's type, and O += P V takes it from there.  The running maximum a
 // row's weights are taken against moves only when the true one has passed it by 2^8 (weights then stay below 2^8, far from
@@ -248,7 +251,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     if (tid == 0) s_seq = 0xFFFFFFFFu;
     if (seqs <= PP_THREADS) {
         PgSeq mine = {};
-        uint32_t n = 0, before = 0;
+        uint32_t n = 0;
+        uint64_t before = 0;
         if (tid < seqs) {
             mine = pg_seq(a, tid);
             n = pp_blocks(pa, mine);
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             }
             if (before <= want && want - before < n) {
                 s_seq = tid;
-                s_before = before + n;
+                s_before = (uint32_t)(before + n);
                 s_found = mine;
             }
         }
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         __syncthreads();
     } else {
         uint32_t* s_sum = reinterpret_cast<uint32_t*>(s_kv);
-        uint32_t before = 0;
+        uint64_t before = 0;
         for (uint32_t b0 = 0; b0 < seqs; b0 += PP_THREADS) {
             const uint32_t b = b0 + tid;
             PgSeq mine = {};
@@ -287,14 +291,14 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             __syncthreads();
             if (lane == 31) s_sum[warp] = incl;
             __syncthreads();
-            uint32_t excl = before + incl - n;
+            uint64_t excl = before + incl - n;
             for (uint32_t i = 0; i < PP_THREADS / 32; i++) {
                 if (i < warp) excl += s_sum[i];
                 before += s_sum[i];
             }
             if (excl <= want && want - excl < n) {
                 s_seq = b;
-                s_before = excl + n;
+                s_before = (uint32_t)(excl + n);
                 s_found = mine;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     const uint32_t all_rows = sq.q_len * a.group, row0 = block * pa.block, rows = min(pa.block, all_rows - row0);
     const uint32_t see = pg_limit(sq, (row0 + rows - 1) / a.group);  // keys the block's last token sees (the most)
     const uint32_t n_all = (see + PP_KEYS - 1) / PP_KEYS;
-    const uint32_t t0 = n_all * split / pa.splits, t1 = n_all * (split + 1) / pa.splits, n = t1 - t0;  // (below 2^24 tiles, at most 148 splits)
+    const uint32_t t0 = n_all * split / pa.splits, t1 = n_all * (split + 1) / pa.splits, n = t1 - t0;  // (below 2^24 tiles, fewer splits than SMs)
     const bool dual = rows <= PP_ROWS;
 
     // ---- Q to shared memory.  Where the group divides 128 the loader asks for whole boxes; otherwise row by row, all of it in
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         bool ok = true;
         uint32_t it = 0;
         for (uint32_t t = t0 + (dual ? w : 0); t < t1; t += dual ? 2 : 1, it++) {
-            if (!(ok = pp_wait(&s_full[w], it & 1, gave_up))) break;
+            if (!(ok = __all_sync(0xFFFFFFFFu, pp_wait(&s_full[w], it & 1, gave_up)))) break;
             pp_after();
             float s[128];
 #pragma unroll
@@ -479,11 +483,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             }
         }
         // ---- epilogue ----
-        if (ok && it) ok = pp_wait(&o_full[w], 0, gave_up);
-        if (ok && dual && w == 1 && n) ok = pp_wait(&o_full[0], 0, gave_up);  // it writes where the other's products read
+        if (ok && it) ok = __all_sync(0xFFFFFFFFu, pp_wait(&o_full[w], 0, gave_up));
+        if (ok && dual && w == 1 && n) ok = __all_sync(0xFFFFFFFFu, pp_wait(&o_full[0], 0, gave_up));  // it writes where the other's products read
         pp_after();
-        // (c is positive; a row that has seen no key may have collected weights of 2^-127)
-        float l = m == -INFINITY ? 0.0f : l0 + l1, ml = m * c;
+        float l = l0 + l1, ml = m * c;  // (-inf stays -inf: c is positive)
         float* other = reinterpret_cast<float*>(sR);  // [HD][128] and then m, l [128] each
         if (dual && w == 1) {
             // its part of the rows, for the first warpgroup; every load of the ring has been read by a product by now
