@@ -390,7 +390,15 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             pp_ld_done();
             const uint32_t key0 = t * PP_KEYS;
             float shift = 0.0f;  // of all the row's scores of this tile
+            const bool masked = key0 + PP_KEYS > lim_warp;
+            const uint32_t left = lim > key0 ? lim - key0 : 0;
             if (SCORED) {
+                if (masked && a.cap_mul != 0.0f) {
+                    // columns that the row does not see may hold anything (the last tile's, what was in shared memory): they
+                    // must not choose the form of the cap
+#pragma unroll
+                    for (uint32_t i = 0; i < 128; i++) s[i] = i < left ? s[i] : 0.0f;
+                }
                 if (before) {
                     const uint64_t mul2 = pp_pack2(a.score_mul);
 #pragma unroll
@@ -429,8 +437,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     }
                 }
             }
-            if (key0 + PP_KEYS > lim_warp) {
-                const uint32_t left = lim > key0 ? lim - key0 : 0;
+            if (masked) {
 #pragma unroll
                 for (uint32_t i = 0; i < 128; i++) s[i] = i < left ? s[i] : -INFINITY;
             }

@@ -367,6 +367,25 @@ def test_other_stream_and_repeatability():
     side.synchronize()
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(cap=20.0), dict(slopes=True), dict(cap=20.0, slopes=True)], ids=str)
+def test_results_do_not_depend_on_what_ran_before(kw):
+    """The same call gives the same bits whatever other calls left in the SMs' shared memory: the last tile of a sequence
+    holds rows that nothing was copied to."""
+    q_lens = kv_lens = [469, 300, 77]
+    m, cache, batch, out = run(55, q_lens, kv_lens, 2, 1, 128, 16, BF, **kw)
+    sl = torch.tensor([2.0 ** (-4.0 * (h + 1)) for h in range(2)], device=DEV) if kw.get("slopes") else None
+    loud = ref.make(56, q_lens, [512, 384, 128], 2, 1, 128, 16, BF)
+    loud_cache = paged.PagedKVCache.from_parts((loud["k"] * 40).to(DEV), loud["v"].to(DEV))
+    loud_batch = paged.PagedBatch(loud_cache, loud["table"].to(DEV), ints([512, 384, 128]), ints(loud["cu"]))
+    q = m["q"].to(DEV)
+    for _ in range(4):
+        paged.paged_attention(loud_batch, loud["q"].to(DEV))
+        assert torch.equal(paged.paged_attention(batch, q, softcap=kw.get("cap", 0.0), slopes=sl), out)
+        quiet = paged.PagedBatch(loud_cache, loud_batch.table, ints([0, 0, 0]), loud_batch.cu_q)
+        paged.paged_attention(quiet, loud["q"].to(DEV))
+        assert torch.equal(paged.paged_attention(batch, q, softcap=kw.get("cap", 0.0), slopes=sl), out)
+
+
 def test_what_the_host_cannot_see_is_reported():
     heads, hd, kv = 4, 128, [20, 70, 3]
     m = ref.make(50, [1, 1, 1], kv, heads, 2, hd, 16, BF, garbage=0.0)
