@@ -280,6 +280,32 @@ def test_append(src, dtype, hd, rot, q_lens, kv_lens):
     cache.check()
 
 
+@pytest.mark.parametrize("src", [torch.float32, BF])
+def test_append_many_tokens_and_unaligned_rows(src):
+    """A prompt of thousands of tokens; the same rows at odd addresses (one element at a time) give the same bits."""
+    heads, kvh, hd, ps, T = 4, 2, 64, 32, 2501
+    table = torch.randperm(90, generator=torch.Generator().manual_seed(1)).to(torch.int32).reshape(1, 90).to(DEV)
+    w = (heads + 2 * kvh) * hd
+    x = torch.randn(T, w, generator=torch.Generator().manual_seed(2)).to(src).to(DEV)
+    odd = torch.empty(T, w + 3, dtype=src, device=DEV)
+    odd[:, 1: 1 + w] = x
+    odd = odd[:, 1: 1 + w]
+    cos, sin = paged.rope_table(T + 9, hd, device=DEV)
+    a, b = heads * hd, (heads + kvh) * hd
+    got = []
+    for y in (x, odd):
+        cache = paged.PagedKVCache(90, ps, kvh, hd, device=DEV)
+        batch = paged.PagedBatch(cache, table, ints([T + 4]), ints([0, T]))
+        got.append((paged.paged_rope_append(batch, y[:, :a], y[:, a:b], y[:, b:], cos, sin), cache.k, cache.v))
+        cache.check()
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+    places = torch.arange(4, T + 4)
+    want, e = ref.rotate(x[:, :a].cpu().double().reshape(T, heads, hd), cos.cpu()[places], sin.cpu()[places])
+    within(got[0][0].reshape(T, heads, hd), want, (2.0 ** -8 * want.abs() + e) * (1 + 2.0 ** -8))
+    page, slot = table.cpu()[0, places // ps].long(), places % ps
+    assert torch.equal(got[0][2].cpu()[page, :, slot].reshape(T, -1), x[:, b:].cpu().to(BF))
+
+
 def test_append_rotates_as_the_single_position_kernel_does():
     """Against decoder.rope_append at one position: the same products, at most one rounding apart."""
     from quanta_b200 import decoder as dec
