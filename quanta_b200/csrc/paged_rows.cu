@@ -1,4 +1,5 @@
-// Paged attention for few rows per K/V head (single tokens, drafts): bounded by the bytes of K and V.
+// Paged attention for few rows per K/V head (single tokens, drafts): bounded by the bytes of K and V (64 sequences of 1 to
+// 8192 keys, 32 / 8 heads of 128: 161 us, 6.6 TB/s; 16 of 1024 keys, 32 / 32 heads: 43 us, 6.2 TB/s).
 //
 // A unit is (sequence of at most 16 packed rows, K/V head); it has ceil(keys / 64) tiles of 64 keys.  The tiles of all
 // units, end to end, are cut into equal runs, one per CTA, so that ragged batches and one long sequence keep every SM
