@@ -919,6 +919,9 @@ static qb200_status launch_prompt(const PpArgs& pa, uint32_t grid, const CUtenso
 qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t splits, uint32_t min_rows, cudaStream_t st) {
     PpEncodeFn enc = pp_encode_fn();
     if (!enc) return fail(QB200_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled is not available from this driver");
+    int dev = 0;  // (the map encoder below needs a current context, which a new thread has only once a device is set)
+    QB_CUDA_TRY(cudaGetDevice(&dev));
+    QB_CUDA_TRY(cudaSetDevice(dev));
     const uint32_t ps = 1u << a.ps_log;
     CUtensorMap map[3];
     for (int i = 0; i < 2; i++) {

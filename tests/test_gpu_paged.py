@@ -393,6 +393,29 @@ def test_other_stream_and_repeatability():
     side.synchronize()
 
 
+@pytest.mark.parametrize("width", [0, WIDE])
+def test_calls_from_new_threads(width):
+    """A thread whose first CUDA work this is, three at a time."""
+    import threading
+    m, cache, batch, out = run(91, [300, 1], [300, 90], 8, 2, width=width)
+    q, seen = m["q"].to(DEV), []
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            seen.append(all(torch.equal(paged.paged_attention(batch, q), out) for _ in range(10)))
+        except Exception as e:
+            seen.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert seen == [True] * 3
+    cache.check()
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(cap=20.0), dict(slopes=True), dict(cap=20.0, slopes=True)], ids=str)
 def test_results_do_not_depend_on_what_ran_before(kw):
     """The same call gives the same bits whatever other calls left in the SMs' shared memory: the last tile of a sequence
