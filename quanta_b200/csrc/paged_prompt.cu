@@ -919,18 +919,24 @@ static qb200_status launch_prompt(const PpArgs& pa, uint32_t grid, const CUtenso
 qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t splits, uint32_t min_rows, cudaStream_t st) {
     PpEncodeFn enc = pp_encode_fn();
     if (!enc) return fail(QB200_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled is not available from this driver");
-    int dev = 0;  // (the map encoder below needs a current context, which a new thread has only once a device is set)
+    int dev = 0;
     QB_CUDA_TRY(cudaGetDevice(&dev));
-    QB_CUDA_TRY(cudaSetDevice(dev));
     const uint32_t ps = 1u << a.ps_log;
     CUtensorMap map[3];
     for (int i = 0; i < 2; i++) {
         const cuuint64_t dims[4] = {hd, ps, a.kv_heads, a.n_pages};
         const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)ps * hd * 2, (cuuint64_t)a.kv_heads * ps * hd * 2};
         const cuuint32_t box[4] = {64, ps < PP_KEYS ? ps : PP_KEYS, 1, 1}, estr[4] = {1, 1, 1, 1};
-        const CUresult cr = enc(&map[i], dtype == QB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                                const_cast<uint16_t*>(i ? a.v : a.k), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        const auto encode = [&] {
+            return enc(&map[i], dtype == QB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                       const_cast<uint16_t*>(i ? a.v : a.k), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        };
+        CUresult cr = encode();
+        if (cr == CUDA_ERROR_INVALID_CONTEXT) {  // a thread without CUDA work so far has no current context until a device is set
+            QB_CUDA_TRY(cudaSetDevice(dev));
+            cr = encode();
+        }
         if (cr != CUDA_SUCCESS) return fail(QB200_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled failed with code " + std::to_string((int)cr));
     }
     PpArgs pa = {};
