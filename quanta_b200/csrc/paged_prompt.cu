@@ -321,8 +321,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     const bool dual = rows <= PP_ROWS;
 
     // ---- Q to shared memory.  Where the group divides 128 the loader asks for whole boxes; otherwise row by row, all of it in
-    // flight at once, and rows past the last one are zeros (1500 cycles of a unit more) ----
-    if (!pa.q_boxes && warp < 8 && (!dual || warp < 4)) {
+    // flight at once, and rows past the last one are zeros (1500 cycles of a unit more).  A unit without keys (a block that sees
+    // none, an empty range of a cut one) has no product that would wait for Q: it brings none, since its results go through the
+    // same shared memory and nothing may be in flight when the CTA ends ----
+    if (!pa.q_boxes && n && warp < 8 && (!dual || warp < 4)) {
         constexpr uint32_t CH = HD / 8, STEP = 128 / CH;
         const uint32_t w = warp >> 2, wt = tid & 127, ch = wt % CH, first = w * PP_ROWS, t_rows = min(PP_ROWS, rows - first);
         const uint32_t whole = STEP / a.group, rest = STEP % a.group;
@@ -582,7 +584,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     for (uint32_t i = 0; i < 8; i++)
                         if ((i0 + i) * (32 / PER) + row_in < n_rows) *reinterpret_cast<uint4*>(a.out + (uint64_t)to[i] * HD + piece * 8) = v[i];
                 }
-            } else {
+            } else if (!parts || n) {  // (a range without keys leaves its m and l alone: nothing is read at weight 0)
                 // partial results and rows that are joined: 32 bits, half of the columns at a time
                 constexpr uint32_t COLS = HD / 2, PER = COLS / 4, N = PER;
                 const uint32_t row_in = lane / PER, piece = lane % PER;
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             count++;
             if (++st == S::STAGES) st = 0;
         };
-        if (pa.q_boxes && lane == 0) {
+        if (pa.q_boxes && n && lane == 0) {
             // (rows behind the sequence's last one are the next sequence's, or zeros: their results are not stored)
             const uint32_t tiles = dual ? 1 : 2;
             pp_expect(q_full, tiles * S::TILE);
