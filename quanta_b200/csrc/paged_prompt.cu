@@ -213,9 +213,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
     uint64_t* p_full = s_full + 2;         // [2][2] half of the tile's P (64 keys) is in TMEM
     uint64_t* o_full = p_full + 4;         // [2] the tile's O is complete
     uint64_t* cleaned = o_full + 2;        // the last tile of V has zeros behind its last key
-    uint64_t* drained = cleaned + 1;       // after giving up: the products in flight are complete
+    uint64_t* drained = cleaned + 1;       // after giving up: every product that was issued is complete
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile uint32_t* gave_up = tmem_slot + 1;
+    volatile uint32_t* loaded = tmem_slot + 2;  // tiles that were asked for
     const PgArgs& a = pa.g;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -694,8 +695,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 if (lane == 0) pp_arrive(cleaned);
             }
         }
-        if (!ok)  // given up: let the copies in flight land before the memory goes
-            for (uint32_t i = count > S::STAGES ? count - S::STAGES : 0; i < count; i++) pp_land(&full[i % S::STAGES], (i / S::STAGES) & 1);
+        if (lane == 0) *loaded = count;
       } else if (warp == 9 && n) {
         // ---- products: one thread waits and issues (its branches are its own; the operands' addresses are constants but
         // for the ring slot) ----
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
 #pragma unroll
                     for (uint32_t tile = 0; tile < 2; tile++) {
                         if (!(ok = values(tile, v_slot, i & 1, i > 0, last))) break;
-                        if (tile == 1) pp_commit(&empty[v_slot]);
+                        if (tile == 1 && !last) pp_commit(&empty[v_slot]);  // (nobody waits for the last one)
                         if (!last) scores(tile, tile, k_slot);
                     }
                     if (ok && !last) pp_commit(&empty[k_slot]);
@@ -775,23 +775,34 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                     if (!(ok = next_value(i, v_slot))) break;
                     if (i + 2 < n && !(ok = next(k_slot))) break;
                     if (!(ok = values(tile, v_slot, (i >> 1) & 1, i > 1, i + 2 >= n))) break;
-                    pp_commit(&empty[v_slot]);
+                    if (i + 1 < n) pp_commit(&empty[v_slot]);
                     if (i + 2 < n) {
                         scores(tile, 0, k_slot);
                         pp_commit(&empty[k_slot]);
                     }
                 }
             }
-            if (!ok) {  // given up: the products in flight read shared memory and TMEM
-                pp_commit(drained);
-                pp_land(drained, 0);
-            }
         }
       }
     }
     pp_before();
     __syncthreads();
-    if (tid == 0 && *gave_up) pg_report(a.status, QB200_ERR_TIMEOUT);
+    if (*gave_up) {
+        // Some role has given up, and all have come here: nobody asks for more, but copies that another role would have waited
+        // for may be on their way into this memory, and products may read it.  (Without a give-up nothing is in flight: every
+        // copy has been waited for by a product, and every product by the epilogue.)
+        if (tid == 0) pg_report(a.status, QB200_ERR_TIMEOUT);
+        if (warp == 8) {
+            const uint32_t count = *loaded;
+            for (uint32_t i = count > S::STAGES ? count - S::STAGES : 0; i < count; i++) pp_land(&full[i % S::STAGES], (i / S::STAGES) & 1);
+            if (pa.q_boxes && n) pp_land(q_full, 0);
+        }
+        if (warp == 9 && pp_elect()) {  // the thread that issued them
+            pp_commit(drained);
+            pp_land(drained, 0);
+        }
+        __syncthreads();
+    }
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
