@@ -289,7 +289,9 @@ QB200_API qb200_status qb200_sum_arrays(const float* parts, uint32_t count, uint
  * qb200_shared_prefix_attention: every token of the batch sees the first prefix_len keys of prefix_pages (page numbers
  *   of the same pools), then its own sequence's keys as above (causal, places counted from prefix_len on).  The prefix
  *   is read once for all tokens.
- * qb200_paged_check: waits for the stream, returns a recorded error once and clears it. */
+ * qb200_paged_check: waits for the stream, returns a recorded error once and clears it.
+ * qb200_paged_set_spin_limit: polls that a wait inside the prompts' kernel spends on a copy or a product before the kernel gives
+ *   up, records QB200_ERR_TIMEOUT and returns; process-wide, read at launch time, 4 Mi (about a second) by default. */
 typedef struct qb200_paged_kv {
     void* k_pages;
     void* v_pages;
@@ -322,6 +324,7 @@ QB200_API qb200_status qb200_shared_prefix_attention(const qb200_paged_kv* kv, c
                                                      uint64_t tokens, uint32_t heads, float scale, float softcap, const float* slopes,
                                                      float* scratch, void* out, float* lse, void* stream);
 QB200_API qb200_status qb200_paged_check(const qb200_paged_kv* kv, void* stream);
+QB200_API qb200_status qb200_paged_set_spin_limit(uint32_t polls);
 
 /* ---- fused all-gather for column-sharded layers (no counterpart in the reference: it has no
  * multi-GPU code, crates/ml/quanta-nn/PARITY.md:76-79) ----

@@ -73,6 +73,7 @@ SIGNATURES = {
     "qb200_shared_prefix_scratch_floats": (u64, [vp, vp, u64, u64, u32]),
     "qb200_shared_prefix_attention": (i32, [vp, vp, vp, u64, vp, u64, u64, u32, ctypes.c_float, ctypes.c_float, vp, vp, vp, vp, vp]),
     "qb200_paged_check": (i32, [vp, vp]),
+    "qb200_paged_set_spin_limit": (i32, [u32]),
     "qb200_peer_alloc": (i32, [u64, P(vp), ctypes.c_char_p]),
     "qb200_peer_open": (i32, [ctypes.c_char_p, P(vp)]),
     "qb200_peer_close": (i32, [vp]),

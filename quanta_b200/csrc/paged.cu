@@ -4,6 +4,7 @@
 // once (8620 tokens, 32 / 8 heads of 128, bf16: 38 us, 5.7 TB/s, 0.87 of measured; 16 tokens: 2.4 us in a graph).  A
 // block takes one token; a thread keeps its eight pairs of angles in registers and walks the heads with them, 16
 // elements (two 16-byte groups, the halves of the rotated pairs) at a time, two heads in flight (three: 39.9 us).
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -235,6 +236,9 @@ qb200_status pg_sms(uint32_t* n) {
     return QB200_OK;
 }
 
+static std::atomic<uint32_t> g_pg_spin_limit{4u << 20};
+uint32_t pg_spin_limit() { return g_pg_spin_limit.load(std::memory_order_relaxed); }
+
 // Which kernels a phase needs: sequences of at most PG_FEW_ROWS packed rows go to one, all others to the other; where
 // only the device knows the lengths, both are launched.
 struct PgPlan {
@@ -447,6 +451,12 @@ qb200_status qb200_shared_prefix_attention(const qb200_paged_kv* kv, const qb200
     a.out = static_cast<uint16_t*>(out);
     a.lse = lse;
     return pg_phase(who, a, kv->dtype, kv->head_dim, sms, phase, s);
+}
+
+qb200_status qb200_paged_set_spin_limit(uint32_t polls) {
+    if (polls == 0) return fail(QB200_ERR_INVALID_PARAM, "qb200_paged_set_spin_limit: the limit must be positive");
+    g_pg_spin_limit.store(polls, std::memory_order_relaxed);
+    return QB200_OK;
 }
 
 qb200_status qb200_paged_check(const qb200_paged_kv* kv, void* stream) {

@@ -209,6 +209,7 @@ __device__ __forceinline__ void pg_emit(const PgArgs& a, uint32_t token, uint32_
 }
 
 qb200_status pg_sms(uint32_t* n);  // SMs of the current device
+uint32_t pg_spin_limit();          // polls of a wait inside the prompt kernel
 // Attention for few rows (paged_rows.cu): how it runs and the floats of partial results that takes.
 struct PgRows {
     bool units;      // a cluster of 2^c_log CTAs per unit of 16 rows, row_tiles of them a sequence and K/V head; otherwise equal runs of all tiles, and a second kernel

@@ -31,7 +31,6 @@ namespace qb {
 constexpr uint32_t PP_THREADS = 384, PP_MORE = 216, PP_LESS = 72;
 static_assert(2 * PP_MORE + PP_LESS == 3 * 168, "the shares add up to what the launch gets");
 constexpr uint32_t PP_KEYS = 128, PP_ROWS = 128;
-constexpr uint32_t PP_POLLS = 1u << 22;
 template <uint32_t HD> struct PpShape {
     static constexpr uint32_t PANEL = 128 * 128;            // 128 rows of 64 elements
     static constexpr uint32_t TILE = PANEL * (HD / 64);     // a Q, K or V tile
@@ -51,9 +50,9 @@ __device__ __forceinline__ void pp_arrive(uint64_t* bar) {
 __device__ __forceinline__ void pp_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(pp_smem(bar)), "r"(bytes) : "memory");
 }
-// Bounded wait for a barrier's phase; gives up at once when another role has.
-__device__ __forceinline__ bool pp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* gave_up) {
-    for (uint32_t i = 0; i < PP_POLLS; i++) {
+// One thread's bounded wait for a barrier's phase; gives up at once when another role has.
+__device__ __forceinline__ bool pp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* gave_up, uint32_t polls) {
+    for (uint32_t i = 0; i < polls; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -67,6 +66,11 @@ __device__ __forceinline__ bool pp_wait(uint64_t* bar, uint32_t parity, volatile
     }
     *gave_up = 1;
     return false;
+}
+// The same for a whole warp, which goes on or gives up as one: a lane that went on to the warp's next barrier without those
+// that ran out of polls would wait there for good.
+__device__ __forceinline__ bool pp_wait_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* gave_up, uint32_t polls) {
+    return __all_sync(0xFFFFFFFFu, pp_wait(bar, parity, gave_up, polls));
 }
 // After giving up: a short wait for what is still in flight.
 __device__ __forceinline__ void pp_land(uint64_t* bar, uint32_t parity) {
@@ -187,6 +191,7 @@ struct PpArgs {
     PgArgs g;
     uint32_t splits, min_rows, block;  // block: rows of a unit, 256 or 128
     uint32_t q_boxes;  // Q by TMA: 128 rows are a box of whole tokens
+    uint32_t polls;    // limit of a wait inside the kernel
     float* parts_acc;  // [splits][tokens * heads][hd] and [splits][tokens * heads][2], splits > 1
     float* parts_ml;
 };
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         bool ok = true;
         uint32_t it = 0;
         for (uint32_t t = t0 + (dual ? w : 0); t < t1; t += dual ? 2 : 1, it++) {
-            if (!(ok = __all_sync(0xFFFFFFFFu, pp_wait(&s_full[w], it & 1, gave_up)))) break;
+            if (!(ok = pp_wait_warp(&s_full[w], it & 1, gave_up, pa.polls))) break;
             pp_after();
             float s[128];
 #pragma unroll
@@ -493,8 +498,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             }
         }
         // ---- epilogue ----
-        if (ok && it) ok = __all_sync(0xFFFFFFFFu, pp_wait(&o_full[w], 0, gave_up));
-        if (ok && dual && w == 1 && n) ok = __all_sync(0xFFFFFFFFu, pp_wait(&o_full[0], 0, gave_up));  // it writes where the other's products read
+        if (ok && it) ok = pp_wait_warp(&o_full[w], 0, gave_up, pa.polls);
+        if (ok && dual && w == 1 && n) ok = pp_wait_warp(&o_full[0], 0, gave_up, pa.polls);  // it writes where the other's products read
         pp_after();
         float l = l0 + l1, ml = m * c;  // (-inf stays -inf: c is positive)
         float* other = reinterpret_cast<float*>(sR);  // [HD][128] and then m, l [128] each
@@ -645,7 +650,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             return p;
         };
         auto load = [&](const CUtensorMap* map, uint32_t t, int32_t page) {
-            if (count >= S::STAGES && !pp_wait(&empty[st], (count / S::STAGES - 1) & 1, gave_up)) { ok = false; return; }
+            if (count >= S::STAGES && !pp_wait_warp(&empty[st], (count / S::STAGES - 1) & 1, gave_up, pa.polls)) { ok = false; return; }
             const uint32_t boxes = min(per, (see - t * PP_KEYS + box - 1) / box);
             if (lane == 0) pp_expect(&full[st], boxes * box * HD * 2);
             __syncwarp();
@@ -686,7 +691,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             // anything there, and 0 * NaN is NaN).  V of the last tile was asked for last; this warp knows its turn of the
             // ring (one that had not followed the ring would take the barrier's earlier turns for it).
             const uint32_t slot = (count - 1) % S::STAGES, valid = see - (t1 - 1) * PP_KEYS;
-            if ((ok = pp_wait(&full[slot], ((count - 1) / S::STAGES) & 1, gave_up))) {
+            if ((ok = pp_wait_warp(&full[slot], ((count - 1) / S::STAGES) & 1, gave_up, pa.polls))) {
                 for (uint32_t i = valid * 8 + lane; i < PP_KEYS * 8; i += 32)
 #pragma unroll
                     for (uint32_t p = 0; p < HD / 64; p++) *reinterpret_cast<uint4*>(sR + slot * S::TILE + p * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
@@ -717,7 +722,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
                 const uint64_t db = v_desc + slot * (S::TILE >> 4);
 #pragma unroll
                 for (uint32_t h = 0; h < 2; h++) {
-                    if (!pp_wait(&p_full[2 * tile + h], parity, gave_up)) return false;
+                    if (!pp_wait(&p_full[2 * tile + h], parity, gave_up, pa.polls)) return false;
                     pp_after();
 #pragma unroll
                     for (uint32_t kk = h * 4; kk < h * 4 + 4; kk++)
@@ -729,7 +734,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             uint32_t st = 0, par = 0;  // the ring's next tile, in the order they were loaded
             auto next = [&](uint32_t& slot) -> bool {
                 slot = st;
-                const bool got = pp_wait(&full[st], par, gave_up);
+                const bool got = pp_wait(&full[st], par, gave_up, pa.polls);
                 if (++st == S::STAGES) {
                     st = 0;
                     par ^= 1;
@@ -738,10 +743,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
             };
             // the last tile of V: the loader clears the rows behind the last key that is seen
             auto next_value = [&](uint32_t i, uint32_t& slot) -> bool {
-                if (i + 1 == n && see < (t0 + n) * PP_KEYS && !pp_wait(cleaned, 0, gave_up)) return false;
+                if (i + 1 == n && see < (t0 + n) * PP_KEYS && !pp_wait(cleaned, 0, gave_up, pa.polls)) return false;
                 return next(slot);
             };
-            bool ok = pp_wait(q_full, 0, gave_up);
+            bool ok = pp_wait(q_full, 0, gave_up, pa.polls);
             uint32_t k_slot = 0, v_slot = 0;
             if (!dual) {
                 ok = ok && next(k_slot);
@@ -967,6 +972,7 @@ qb200_status pg_prompt_launch(const PgArgs& a, int dtype, uint32_t hd, uint32_t 
     }
     pa.splits = splits;
     pa.min_rows = min_rows;
+    pa.polls = pg_spin_limit();
     pa.parts_acc = a.parts;
     pa.parts_ml = a.parts + (uint64_t)splits * a.tokens * a.group * a.kv_heads * hd;
     uint32_t sms = 0;

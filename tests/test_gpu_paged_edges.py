@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+import quanta_b200 as qb
+from quanta_b200 import _lib as L
 from quanta_b200 import paged
 from tests import paged_reference as ref
 
@@ -106,3 +108,51 @@ def test_ranges_without_keys(heads, kv_heads):
     want, _, tol, _ = ref.attention(m["q"], m["k"], m["v"], m["table"], kv_lens, m["cu"], heads, 1.0 / math.sqrt(128))
     within(a, want, tol)
     within(b, want, tol)
+
+
+@pytest.fixture()
+def no_patience():
+    lib = L.load()
+    assert lib.qb200_paged_set_spin_limit(1) == 0
+    yield lib
+    assert lib.qb200_paged_set_spin_limit(4 << 20) == 0
+
+
+def test_spin_limit_setter_rejects_zero():
+    assert L.load().qb200_paged_set_spin_limit(0) == L.ERR_INVALID_PARAM and "positive" in L.last_error()
+
+
+# one tile of rows and two, keys in one range and in several, Q by boxes and row by row, behind a prefix
+@pytest.mark.parametrize("heads,kv_heads,q_lens,hd,dtype,width,prefix", [
+    (8, 2, [300, 70], 128, BF, 0, 0), (8, 2, [300, 70], 64, FP, 2500, 0), (6, 2, [400, 1], 128, BF, 0, 0), (16, 16, [700, 500, 300], 64, FP, 0, 0),
+    (24, 8, [500, 513], 128, BF, 0, 0), (8, 2, [300, 70], 128, BF, 0, 700)])
+def test_waits_that_run_out_are_reported(no_patience, heads, kv_heads, q_lens, hd, dtype, width, prefix):
+    """With a single poll per wait the kernel gives up wherever a copy or a product is not there yet: it returns, the status says
+    so once, and the next calls are as they were."""
+    lib = no_patience
+    kv_lens = [n + 5 for n in q_lens]
+    m = ref.make(23, q_lens, kv_lens, heads, kv_heads, hd, 16, dtype, prefix=prefix, width=width)
+    cache, batch = build(m, kv_lens)
+    q, pages = m["q"].to(DEV), m["pre"].to(DEV)
+
+    def call():
+        return paged.shared_prefix_attention(batch, q, pages, prefix) if prefix else paged.paged_attention(batch, q)
+
+    lib.qb200_paged_set_spin_limit(4 << 20)
+    want = call()
+    cache.check()
+    ran_out = 0
+    for _ in range(5):
+        lib.qb200_paged_set_spin_limit(1)
+        got = call()
+        try:
+            cache.check()
+            assert torch.equal(got, want)
+        except qb.QuantError as e:
+            assert e.code == L.ERR_TIMEOUT and "wait ran out" in str(e)
+            ran_out += 1
+        cache.check()  # reported once
+        lib.qb200_paged_set_spin_limit(4 << 20)
+        assert torch.equal(call(), want)
+        cache.check()
+    assert ran_out
