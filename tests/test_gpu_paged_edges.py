@@ -156,3 +156,51 @@ def test_waits_that_run_out_are_reported(no_patience, heads, kv_heads, q_lens, h
         assert torch.equal(call(), want)
         cache.check()
     assert ran_out
+
+
+def capped(m, kv_lens, heads, cap, scale, prefix=0):
+    """The definition in float64 with caps of any size: (out, bound of |out - exact|), causal.
+
+    The bound is that of paged_reference.attention but for the cap, whose error is relative to the score, not to the cap: with
+    x = score / cap, below |x| = 0.3 a polynomial of relative error 2e-6 at most (its best fit's 1.9e-6, four roundings), above it
+    1 - 2 / (e^2x + 1) of absolute error 2^-21 (exponential 2^-22, half of it reaches the result; reciprocal, sums 2^-23 each), which is 1.7e-6 of
+    tanh(0.3): below 2^-18 |score| in all."""
+    hd, kvh = m["k"].shape[3], m["k"].shape[1]
+    group, u, dt = heads // kvh, ref.HALF_STEP[m["k"].dtype], m["k"].dtype
+    q = m["q"].to(ref.F64).reshape(-1, heads, hd)
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    pre = [ref.keys_of(p, m["pre"], prefix) for p in (m["k"], m["v"])]
+    for b, n in enumerate(kv_lens):
+        kk, vv = (torch.cat([x, ref.keys_of(p, m["table"][b], n)], 1) for x, p in zip(pre, (m["k"], m["v"])))
+        lo, hi = m["cu"][b], m["cu"][b + 1]
+        for t in range(lo, hi):
+            see = prefix + n - (hi - lo) + (t - lo) + 1
+            for h in range(heads):
+                K, V = kk[h // group, :see], vv[h // group, :see]
+                s = K @ q[t, h] * scale
+                e = float((hd + 8) * 2.0 ** -24 * abs(scale) * (K.abs() @ q[t, h].abs()).max())
+                s = cap * torch.tanh(s / cap)
+                e += float((2.0 ** -18 + 2.0 ** -21) * s.abs().max())
+                p = torch.softmax(s, 0)
+                out[t, h] = p @ V
+                A = p @ V.abs()
+                tol[t, h] = u * out[t, h].abs() + (u + 2 * e + 2 * (see / 16 + 64) * 2.0 ** -24 + 2.0 ** -20) * (1 + u) * A
+                if dt == FP:
+                    tol[t, h] += see * 2.0 ** -25 * V.abs().max() + 2.0 ** -25
+    return out.reshape(-1, heads * hd), tol.reshape(-1, heads * hd)
+
+
+@pytest.mark.parametrize("cap", [1e-6, 0.5, 30.0, 1e3, 1e5, 1e6, 1e8, 1e20])
+@pytest.mark.parametrize("q_lens,kv_lens,heads,prefix", [([1, 1, 1], [40, 1, 300], 4, 0), ([3, 1], [9, 170], 4, 70), ([270, 3], [270, 90], 8, 0)])
+def test_caps_of_every_size(q_lens, kv_lens, heads, prefix, cap):
+    """A cap far above the scores leaves them as they are, in the kernels for few rows as in the one for prompts."""
+    for hd, dtype, scale, width in ((128, BF, None, 0), (64, FP, 0.4, 2500)):
+        m = ref.make(29, q_lens, kv_lens, heads, 2, hd, 16, dtype, prefix=prefix, width=width)
+        cache, batch = build(m, kv_lens)
+        q = m["q"].to(DEV)
+        if prefix:
+            out = paged.shared_prefix_attention(batch, q, m["pre"].to(DEV), prefix, scale=scale, softcap=cap)
+        else:
+            out = paged.paged_attention(batch, q, scale=scale, softcap=cap)
+        cache.check()
+        within(out, *capped(m, kv_lens, heads, cap, 1.0 / math.sqrt(hd) if scale is None else scale, prefix))
