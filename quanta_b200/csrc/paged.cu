@@ -291,6 +291,9 @@ static qb200_status pg_phase(const char* who, PgArgs a, int dtype, uint32_t hd, 
 }
 
 static void pg_scores(PgArgs& a, float scale, float softcap, const float* slopes) {
+    // cap * log2 e and scale / cap leave the range of 32 bits for the largest caps, which do nothing: past 1e30 the cap takes less
+    // than half a step from any score below 1e26
+    if (softcap > 1e30f) softcap = 0.0f;
     a.score_mul = softcap > 0.0f ? scale / softcap : scale * PG_LOG2E;
     a.cap_mul = softcap > 0.0f ? softcap * PG_LOG2E : 0.0f;
     a.slopes = slopes;

@@ -204,3 +204,14 @@ def test_caps_of_every_size(q_lens, kv_lens, heads, prefix, cap):
             out = paged.paged_attention(batch, q, scale=scale, softcap=cap)
         cache.check()
         within(out, *capped(m, kv_lens, heads, cap, 1.0 / math.sqrt(hd) if scale is None else scale, prefix))
+
+
+@pytest.mark.parametrize("cap", [2e30, 1e38, 3.4e38])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [40, 300]), ([270, 3], [270, 90])])
+def test_the_largest_caps(q_lens, kv_lens, cap):
+    """Near the end of the 32-bit range the cap does nothing."""
+    m = ref.make(30, q_lens, kv_lens, 8, 2, 128, 16, BF)
+    cache, batch = build(m, kv_lens)
+    q = m["q"].to(DEV)
+    assert torch.equal(paged.paged_attention(batch, q, softcap=cap), paged.paged_attention(batch, q))
+    cache.check()
