@@ -239,5 +239,5 @@ def shared_prefix_attention(batch: PagedBatch, q: torch.Tensor, prefix_pages: to
     lib = L.load()
     scratch = _scratch("shared_prefix_attention", batch, scratch, lib.qb200_shared_prefix_scratch_floats, prefix_len, tokens, heads)
     _run(cache, lib.qb200_shared_prefix_attention, cache._ref, batch._ref, prefix_pages.data_ptr(), prefix_len, q.data_ptr(), qs, tokens, heads,
-         cache._scale if scale is None else scale, softcap, sl, scratch.data_ptr(), out.data_ptr(), lp)
+         cache._scale if scale is None else scale, softcap, sl, 0 if scratch is None else scratch.data_ptr(), out.data_ptr(), lp)
     return out

@@ -215,3 +215,12 @@ def test_the_largest_caps(q_lens, kv_lens, cap):
     q = m["q"].to(DEV)
     assert torch.equal(paged.paged_attention(batch, q, softcap=cap), paged.paged_attention(batch, q))
     cache.check()
+
+
+@pytest.mark.parametrize("width", [0, 2500])
+def test_no_tokens_behind_a_shared_prefix(width):
+    m = ref.make(33, [0, 0], [20, 9], 4, 2, 128, 16, BF, prefix=40, width=width)
+    cache, batch = build(m, [20, 9])
+    q = torch.empty(0, 512, dtype=BF, device=DEV)
+    assert paged.shared_prefix_attention(batch, q, m["pre"].to(DEV), 40).shape == (0, 512)
+    cache.check()
