@@ -189,15 +189,29 @@ static qb200_status pg_check_cache(const char* who, const qb200_paged_kv* kv, co
     return QB200_OK;
 }
 
+static qb200_status pg_check_heads(const char* who, const qb200_paged_kv* kv, uint64_t tokens, uint32_t heads) {
+    const std::string w(who);
+    if (heads == 0 || heads % kv->kv_heads)
+        return fail(QB200_ERR_INVALID_PARAM, w + ": " + std::to_string(heads) + " heads are no multiple of " + std::to_string(kv->kv_heads) + " K/V heads");
+    if (tokens * heads > 0x7FFFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, w + ": 2^31 query rows or more");
+    return QB200_OK;
+}
+
+static qb200_status pg_check_prefix(const char* who, const qb200_paged_kv* kv, const qb200_paged_batch* b, uint64_t prefix_len) {
+    const std::string w(who);
+    if (prefix_len == 0) return fail(QB200_ERR_INVALID_PARAM, w + ": no prefix (call qb200_paged_attention)");
+    if (prefix_len > 0x7FFFFFFFull || prefix_len + (uint64_t)b->table_width * kv->page_size > 0x7FFFFFFFull)
+        return fail(QB200_ERR_NOT_SUPPORTED, w + ": 2^31 keys or more");
+    return QB200_OK;
+}
+
 static qb200_status pg_check_attention(const char* who, const qb200_paged_kv* kv, const qb200_paged_batch* b, const void* q, uint64_t q_stride,
                                        uint64_t tokens, uint32_t heads, float scale, float softcap, const float* scratch, const void* out) {
     qb200_status st = pg_check_cache(who, kv, b, tokens);
     if (st) return st;
     const std::string w(who);
     if (tokens && (!q || !out)) return fail(QB200_ERR_INVALID_PARAM, w + ": null pointer");
-    if (heads == 0 || heads % kv->kv_heads)
-        return fail(QB200_ERR_INVALID_PARAM, w + ": " + std::to_string(heads) + " heads are no multiple of " + std::to_string(kv->kv_heads) + " K/V heads");
-    if (tokens * heads > 0x7FFFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, w + ": 2^31 query rows or more");
+    if ((st = pg_check_heads(who, kv, tokens, heads))) return st;
     if (q_stride < (uint64_t)heads * kv->head_dim || q_stride % 8) return fail(QB200_ERR_LENGTH, w + ": q's row stride must be a multiple of 8 that holds all heads");
     if (!pg_aligned(q, 16) || !pg_aligned(out, 16) || !pg_aligned(scratch, 16))
         return fail(QB200_ERR_INVALID_PARAM, w + ": q, out and scratch must be 16-byte aligned");
@@ -379,8 +393,9 @@ qb200_status qb200_paged_rope_append(const qb200_paged_kv* kv, const qb200_paged
 }
 
 uint64_t qb200_paged_attention_scratch_floats(const qb200_paged_kv* kv, const qb200_paged_batch* batch, uint64_t tokens, uint32_t heads) {
+    const char* who = "qb200_paged_attention_scratch_floats";
     uint32_t sms = 0;
-    if (!kv || !batch || kv->kv_heads == 0 || pg_sms(&sms)) return 0;
+    if (pg_check_cache(who, kv, batch, tokens) || pg_check_heads(who, kv, tokens, heads) || pg_sms(&sms)) return 0;
     return pg_plan(pg_args(kv, batch, tokens, heads), kv->head_dim, sms).floats;
 }
 
@@ -420,8 +435,9 @@ static uint64_t prefix_rows_floats(const PgArgs& a, uint32_t hd) { return ((uint
 
 uint64_t qb200_shared_prefix_scratch_floats(const qb200_paged_kv* kv, const qb200_paged_batch* batch, uint64_t prefix_len, uint64_t tokens,
                                             uint32_t heads) {
+    const char* who = "qb200_shared_prefix_scratch_floats";
     uint32_t sms = 0;
-    if (!kv || !batch || kv->kv_heads == 0 || pg_sms(&sms)) return 0;
+    if (pg_check_cache(who, kv, batch, tokens) || pg_check_heads(who, kv, tokens, heads) || pg_check_prefix(who, kv, batch, prefix_len) || pg_sms(&sms)) return 0;
     const PgArgs own = pg_args(kv, batch, tokens, heads);
     const uint64_t x = pg_plan(own, kv->head_dim, sms).floats;
     const uint64_t y = pg_plan(prefix_args(own, nullptr, prefix_len, kv->head_dim, nullptr), kv->head_dim, sms).floats;
@@ -434,9 +450,8 @@ qb200_status qb200_shared_prefix_attention(const qb200_paged_kv* kv, const qb200
     const char* who = "qb200_shared_prefix_attention";
     qb200_status st = pg_check_attention(who, kv, batch, q, q_stride, tokens, heads, scale, softcap, scratch, out);
     if (st) return st;
-    if (!prefix_pages || prefix_len == 0) return fail(QB200_ERR_INVALID_PARAM, std::string(who) + ": no prefix (call qb200_paged_attention)");
-    if (prefix_len + (uint64_t)batch->table_width * kv->page_size > 0x7FFFFFFFull)
-        return fail(QB200_ERR_NOT_SUPPORTED, std::string(who) + ": 2^31 keys or more");
+    if (!prefix_pages) return fail(QB200_ERR_INVALID_PARAM, std::string(who) + ": no prefix (call qb200_paged_attention)");
+    if ((st = pg_check_prefix(who, kv, batch, prefix_len))) return st;
     if (tokens == 0) return QB200_OK;
     uint32_t sms = 0;
     if ((st = pg_sms(&sms))) return st;

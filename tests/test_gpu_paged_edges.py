@@ -1,4 +1,5 @@
 """The paged cache's operators where their calls are at an edge: units without keys, padding, caps of every size, odd row starts."""
+import ctypes
 import math
 
 import pytest
@@ -224,3 +225,27 @@ def test_no_tokens_behind_a_shared_prefix(width):
     q = torch.empty(0, 512, dtype=BF, device=DEV)
     assert paged.shared_prefix_attention(batch, q, m["pre"].to(DEV), 40).shape == (0, 512)
     cache.check()
+
+
+def test_workspace_sizes_of_refused_calls():
+    """0 and a message, whatever the descriptions hold; nothing is read through their pointers."""
+    lib, P = L.load(), 1 << 20
+    good, seqs = dict(n_pages=10, page_size=16, kv_heads=2, head_dim=128, dtype=L.BF16), dict(table_stride=8, table_width=8, batch=3)
+
+    def sizes(kv=(), b=(), tokens=5, heads=4, prefix=20):
+        c = L.PagedKv(k_pages=P, v_pages=P, status_dev=P, **{**good, **dict(kv)})
+        s = L.PagedBatch(table=P, kv_lens=P, cu_q=P, **{**seqs, **dict(b)})
+        c, s = ctypes.byref(c), ctypes.byref(s)
+        return lib.qb200_paged_attention_scratch_floats(c, s, tokens, heads), lib.qb200_shared_prefix_scratch_floats(c, s, prefix, tokens, heads)
+
+    assert sizes()[1] > 0
+    assert sizes(b=dict(table_width=2500, table_stride=2500), tokens=1000)[0] > 0  # keys cut into ranges
+    for kw in (dict(b=dict(batch=0)), dict(b=dict(table_width=0)), dict(b=dict(table_stride=7)), dict(b=dict(table_width=1 << 28, table_stride=1 << 28)),
+               dict(kv=dict(page_size=0)), dict(kv=dict(page_size=48)), dict(kv=dict(page_size=0xFFFFFFFF)), dict(kv=dict(kv_heads=0)), dict(kv=dict(head_dim=0)),
+               dict(kv=dict(n_pages=0)), dict(kv=dict(dtype=L.F32)), dict(heads=0), dict(heads=3), dict(tokens=1 << 28), dict(tokens=1 << 27, heads=64)):
+        assert sizes(**kw) == (0, 0), kw
+        assert "scratch_floats" in L.last_error()
+    for n in (0, 1 << 31, (1 << 31) - 128, (1 << 64) - 1):
+        assert sizes(prefix=n)[1] == 0, n
+        assert "qb200_shared_prefix_scratch_floats" in L.last_error()
+    assert lib.qb200_paged_attention_scratch_floats(None, None, 5, 4) == 0 and lib.qb200_shared_prefix_scratch_floats(None, None, 20, 5, 4) == 0
