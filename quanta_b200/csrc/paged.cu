@@ -202,6 +202,7 @@ static qb200_status pg_check_prefix(const char* who, const qb200_paged_kv* kv, c
     if (prefix_len == 0) return fail(QB200_ERR_INVALID_PARAM, w + ": no prefix (call qb200_paged_attention)");
     if (prefix_len > 0x7FFFFFFFull || prefix_len + (uint64_t)b->table_width * kv->page_size > 0x7FFFFFFFull)
         return fail(QB200_ERR_NOT_SUPPORTED, w + ": 2^31 keys or more");
+    if (kv->kv_heads * ((prefix_len + 63) / 64) > 0xFFFFFFFFull) return fail(QB200_ERR_NOT_SUPPORTED, w + ": the prefix spans 2^32 tiles of 64 keys or more");
     return QB200_OK;
 }
 

@@ -42,3 +42,15 @@ def test_prefixes_past_the_range():
     for n in (0, 1 << 31, (1 << 31) - 128, (1 << 64) - 1):
         assert prefix_size(n=n) == 0
         assert L.last_error().startswith("qb200_shared_prefix_scratch_floats"), n
+
+
+def test_tiles_of_a_prefix_are_counted_in_32_bits():
+    """All K/V heads' tiles of 64 keys: refused from 2^32 on, as a table's are."""
+    c = kv(kv_heads=1024)
+
+    def call(n):
+        return lib.qb200_shared_prefix_attention(ctypes.byref(c), ctypes.byref(seqs()), P, n, P, 1024 * 128, 5, 1024, 0.1, 0.0, None, None, 2 * P, None, None)
+
+    assert call(1 << 28) == L.ERR_NOT_SUPPORTED and "2^32 tiles" in L.last_error()
+    assert call((1 << 28) - 63) == L.ERR_NOT_SUPPORTED and "2^32 tiles" in L.last_error()
+    assert "2^32 tiles" not in (call((1 << 28) - 64), L.last_error())[1]  # one tile a head fewer
