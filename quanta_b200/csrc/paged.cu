@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(128) k_paged_append(const AppendArgs a) {
         if (b >= a.batch) return;  // a row behind the last sequence
         lo = a.cu_q[b];
         hi = a.cu_q[b + 1];
+        if (b == 0 && (int32_t)t < lo && lo <= hi && hi <= (int32_t)a.tokens) return;  // a row before the first sequence
     }
     const int32_t kv = a.kv_lens[b];
     // (a 32-bit kv and hi - lo in [1, tokens]: no overflow in 64 bits)

@@ -249,3 +249,39 @@ def test_workspace_sizes_of_refused_calls():
         assert sizes(prefix=n)[1] == 0, n
         assert "qb200_shared_prefix_scratch_floats" in L.last_error()
     assert lib.qb200_paged_attention_scratch_floats(None, None, 5, 4) == 0 and lib.qb200_shared_prefix_scratch_floats(None, None, 20, 5, 4) == 0
+
+
+@pytest.mark.parametrize("q_lens", [[3, 1], [200, 130]])
+@pytest.mark.parametrize("before", [1, 5, 150])
+def test_rows_before_the_first_sequence(q_lens, before):
+    """cu_q that does not begin at 0: the rows before it belong to nobody, in append as in both attentions, and nothing is reported."""
+    heads, kvh, hd, prefix, kv_lens = 8, 2, 128, 50, [n + 20 for n in q_lens]
+    m = ref.make(35, q_lens, kv_lens, heads, kvh, hd, 16, BF, garbage=0.5, prefix=prefix)
+    cache, batch = build(m, kv_lens)
+    rows, a, c = m["cu"][-1], heads * hd, (heads + kvh) * hd
+    x = torch.randn(before + rows + 2, (heads + 2 * kvh) * hd, generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    y = x[before: before + rows]
+    late = paged.PagedBatch(cache, batch.table, batch.kv_lens, batch.cu_q + before)
+    cos, sin = paged.rope_table(400, hd, device=DEV)
+    own = slice(before, before + rows)
+
+    def left(t):
+        return (t[:before] == 77.0).all() and (t[before + rows:] == 77.0).all()
+
+    q = paged.paged_rope_append(batch, y[:, :a], y[:, a:c], y[:, c:], cos, sin)
+    k, v = cache.k.clone(), cache.v.clone()
+    cache.k.copy_(m["k"])
+    cache.v.copy_(m["v"])
+    q2 = torch.full((x.shape[0], a), 77.0, dtype=BF, device=DEV)
+    paged.paged_rope_append(late, x[:, :a], x[:, a:c], x[:, c:], cos, sin, q_out=q2)
+    cache.check()
+    assert torch.equal(q2[own], q) and left(q2) and torch.equal(cache.k, k) and torch.equal(cache.v, v)
+    for call in (lambda b, q, **kw: paged.paged_attention(b, q, **kw), lambda b, q, **kw: paged.shared_prefix_attention(b, q, m["pre"].to(DEV), prefix, **kw)):
+        out, lse = torch.full_like(q2, 77.0), torch.full((x.shape[0], heads), 77.0, device=DEV)
+        call(late, q2, out=out, lse=lse)
+        cache.check()
+        want = call(batch, q)
+        # (the other row of a tile, and the other number of rows, may change how a row's keys are cut and joined)
+        assert ((out[own].double() - want.double()).abs() <= 4 * 2.0 ** -8 * float(v.float().abs().max())).all()
+        assert left(out) and left(lse)
+    cache.check()
