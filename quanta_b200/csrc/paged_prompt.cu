@@ -385,7 +385,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
         const float c = SCORED && a.cap_mul != 0.0f ? a.cap_mul : before ? 1.0f : a.score_mul;
         const uint64_t c2 = pp_pack2(c);
         if (SCORED) slope *= PG_LOG2E / c;  // in units of what the exponential scales
-        const float slack = 8.0f / c;  // 2^8 in units of the score (c is positive)
+        // 2^8 in units of the score (c is positive).  Q of a row past the last one may be anything (the next sequence's, or
+        // nobody's): it has no say in what its warp does, so that nothing of it reaches the others' bits.
+        const float slack = r < t_rows ? 8.0f / c : INFINITY;
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         bool ok = true;
         uint32_t it = 0;
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) k_paged_prompt(const __grid_con
 #pragma unroll
                         for (uint32_t k = 0; k < 4; k++) far[k] = fmaxf(fmaxf(far[k], fabsf(s[i + k])), fabsf(s[i + 4 + k]));
                     const float b = a.score_mul;
-                    if (__any_sync(0xFFFFFFFFu, !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * fabsf(b) <= 0.3f && fabsf(b) <= 64.0f))) {  // (b^5 stays in range)
+                    if (__any_sync(0xFFFFFFFFu, slack != INFINITY && !(fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * fabsf(b) <= 0.3f && fabsf(b) <= 64.0f))) {  // (b^5 stays in range)
 #pragma unroll
                         for (uint32_t i = 0; i < 128; i++) s[i] = pg_cap(s[i] * b, 1.0f);
                     } else {

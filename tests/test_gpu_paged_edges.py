@@ -285,3 +285,24 @@ def test_rows_before_the_first_sequence(q_lens, before):
         assert ((out[own].double() - want.double()).abs() <= 4 * 2.0 ** -8 * float(v.float().abs().max())).all()
         assert left(out) and left(lse)
     cache.check()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=40.0), dict(softcap=1e4)], ids=str)
+@pytest.mark.parametrize("heads,kv_heads,hd,dtype", [(4, 4, 128, BF), (8, 2, 64, FP), (6, 2, 128, BF)])
+def test_rows_of_nobody_and_of_others_change_no_bit(heads, kv_heads, hd, dtype, kw):
+    """A padded batch: the rows behind the last sequence hold anything, and so do the next sequence's; both share tiles with the
+    rows before them."""
+    q_lens, kv_lens, tail = [300, 77, 300], [333, 90, 300], 60
+    m = ref.make(37, q_lens, kv_lens, heads, kv_heads, hd, 16, dtype, tail=tail)
+    cache, batch = build(m, kv_lens)
+    q = m["q"].to(DEV) * 0.5
+    rows, first = sum(q_lens), q_lens[0]
+    want = paged.paged_attention(batch, q, **kw)
+    for junk in (float("nan"), float("inf"), 300.0, 0.0):
+        q[rows:] = junk
+        assert torch.equal(paged.paged_attention(batch, q, **kw)[:rows], want[:rows]), junk
+    for junk in (float("nan"), 300.0, 0.0):
+        q[first: first + q_lens[1]] = junk
+        got = paged.paged_attention(batch, q, **kw)
+        assert torch.equal(got[:first], want[:first]) and torch.equal(got[first + q_lens[1]: rows], want[first + q_lens[1]: rows]), junk
+    cache.check()
