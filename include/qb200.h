@@ -263,7 +263,8 @@ QB200_API qb200_status qb200_sum_arrays(const float* parts, uint32_t count, uint
  *   table_width).  kv_lens counts the call's new tokens.  cu_q [batch + 1]: the new tokens of sequence b are rows
  *   [cu_q[b], cu_q[b + 1]) of the call's arrays, and they are the sequence's last ones; NULL: one new token per sequence
  *   (then tokens == batch).  Rows before cu_q[0] and from cu_q[batch] on belong to nobody and are left as they are in every output.
- *   All of it lives on the device and is read there: a captured call follows later contents.
+ *   All of it lives on the device and is read there: a captured call follows later contents.  It must not change
+ *   while a call that reads it runs.
  * A length that does not fit the call (negative, more keys than the table holds, cu_q falling or past `tokens`) is cut
  * to what fits, a page number outside the pool reads as zeros and is not written, and a position outside the table of
  * angles takes its last row; each is recorded in status_dev, reported once by qb200_paged_check, and the results of

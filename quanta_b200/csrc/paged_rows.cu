@@ -83,12 +83,16 @@ constexpr uint32_t PR_KEPT = PR_WARPS * 32;
 // The CTA's run of tiles, [run0, run1) of the total, and the sequence that holds tile run0 (first: its first tile).
 // Runs differ by at most one tile, the longer ones first.
 struct PrRun {
+    PgSeq s;
     uint32_t run0, run1, first, seq;
     uint32_t base, extra;  // tiles of the shorter runs, how many runs are one longer
 };
-// All threads of the CTA take part; false where it has no run (the same for all).
+// All threads of the CTA take part; false where it has no run (the same for all).  Long batches' lengths are read twice, for the total
+// and to find the run: what is found is kept as it was found, and where another stream's writes in between leave nothing to find
+// there is no run.
 __device__ __forceinline__ bool pr_find_run(const PgArgs& a, uint32_t seqs, PgSeq* kept, PrRun& r) {
     __shared__ uint32_t s_warp[PR_WARPS], s_first, s_seq;
+    __shared__ PgSeq s_found;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     PgSeq mine = {};
     uint32_t sum = 0, w0 = 0;
@@ -118,7 +122,15 @@ __device__ __forceinline__ bool pr_find_run(const PgArgs& a, uint32_t seqs, PgSe
     r.run1 = r.run0 + r.base + (i < r.extra ? 1 : 0);
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < seqs; b0 += PR_KEPT) {
-        const uint32_t b = b0 + tid, w = b0 == 0 ? w0 : b < seqs ? pr_weight(a, pg_seq(a, b)) : 0;
+        const uint32_t b = b0 + tid;
+        uint32_t w = w0;
+        if (b0) {
+            w = 0;
+            if (b < seqs) {
+                mine = pg_seq(a, b);
+                w = pr_weight(a, mine);
+            }
+        }
         uint32_t incl = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -137,10 +149,16 @@ __device__ __forceinline__ bool pr_find_run(const PgArgs& a, uint32_t seqs, PgSe
         if (excl <= r.run0 && r.run0 - excl < w) {
             s_seq = b;
             s_first = excl;
+            s_found = mine;
         }
         __syncthreads();
         if (s_seq != 0xFFFFFFFFu) break;
     }
+    if (s_seq == 0xFFFFFFFFu) {
+        if (tid == 0) pg_report(a.status, QB200_ERR_LENGTH);
+        return false;
+    }
+    r.s = s_found;
     r.seq = s_seq;
     r.first = s_first;
     return true;
@@ -380,7 +398,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
 
     PrAt here, ahead;  // what is computed and what is fetched
     here.b = run.seq;
-    here.s = pr_seq(a, kept, run.seq);
+    here.s = run.s;
     here.tiles = pr_tiles(here.s);
     here.kvh = (run.run0 - run.first) / here.tiles;
     here.t = run.run0 - run.first - here.kvh * here.tiles;
@@ -458,7 +476,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
             meta[2] = (int32_t)sq.q0;
             meta[3] = (int32_t)rows;
             meta[4] = (int32_t)kvh;
-            meta[0] = (int32_t)(x < cut ? x / (run.base + 1) : run.extra + (x - cut) / run.base);  // the CTA that has its last tile
+            // the CTA that has its last tile (one of the grid's, whatever the lengths have become)
+            meta[0] = (int32_t)min(x < cut ? x / (run.base + 1) : run.extra + (x - cut) / run.base, gridDim.x - 1);
         }
         constexpr uint32_t PER = HD / 4;  // threads of a row
         for (uint32_t p0 = 0; p0 < rows; p0 += S::PASS) {

@@ -86,7 +86,7 @@ class PagedBatch:
     call's new tokens included) and, unless every sequence has exactly one new token, ``cu_q [batch + 1]`` (sequence b's
     new tokens are rows ``cu_q[b]:cu_q[b + 1]`` of the call's arrays; rows outside ``cu_q[0]:cu_q[batch]`` belong to nobody and are
     left as they are in every output); int32 on the cache's device.  The tensors are kept, so their contents may change
-    between calls; a batch can be used for the whole life of a set of slots."""
+    between calls (in stream order: not while a call that reads them runs); a batch can be used for the whole life of a set of slots."""
 
     def __init__(self, cache: PagedKVCache, table: torch.Tensor, kv_lens: torch.Tensor, cu_q: Optional[torch.Tensor] = None):
         _want(table.dim() == 2 and kv_lens.dim() == 1 and (cu_q is None or cu_q.dim() == 1), "PagedBatch: table [batch, width], kv_lens [batch], cu_q [batch + 1]",
