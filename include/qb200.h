@@ -284,9 +284,10 @@ QB200_API qb200_status qb200_sum_arrays(const float* parts, uint32_t count, uint
  *   reads K/V head h / (heads / kv_heads).  q [tokens, heads * head_dim] of the cache's type (rows q_stride elements
  *   apart, a multiple of 8; 16-byte aligned), out [tokens, heads * head_dim] dense, not overlapping q; lse [tokens, heads] f32 or NULL: log of the sum of
  *   exp(score).  A row that sees no key gives zeros and -inf.  f32 softmax and accumulation; the softmax weights enter the second
- *   product in the cache's type.  scratch: qb200_paged_attention_scratch_floats floats (0: none, may be NULL; also 0 where the call would be refused), 16-byte aligned, not
+ *   product as two numbers of the cache's type in the kernels for few rows, and rounded to it in the prompts' one.  scratch:
+ *   qb200_paged_attention_scratch_floats floats (0: none, may be NULL; also 0 where the call would be refused), 16-byte aligned, not
  *   shared with a call that may overlap.  A key or value of a sequence that is not finite reaches every row that is computed in
- *   a tile with it, masked there or not; rows behind a sequence's last key may hold anything.
+ *   a tile with it, masked there or not, and leaves NaN or an infinity there; rows behind a sequence's last key may hold anything.
  * qb200_shared_prefix_attention: every token of the batch sees the first prefix_len keys of prefix_pages (page numbers
  *   of the same pools), then its own sequence's keys as above (causal, places counted from prefix_len on).  The prefix
  *   is read once for all tokens.

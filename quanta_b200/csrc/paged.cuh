@@ -146,6 +146,7 @@ template <> struct PgType<__nv_bfloat16> {
         return r;
     }
     static __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+    static __device__ __forceinline__ float2 widen2(uint32_t b) { return make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)); }
 };
 template <> struct PgType<__half> {
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -154,6 +155,7 @@ template <> struct PgType<__half> {
         return r;
     }
     static __device__ __forceinline__ float widen(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+    static __device__ __forceinline__ float2 widen2(uint32_t b) { return make_float2(widen((uint16_t)(b & 0xFFFFu)), widen((uint16_t)(b >> 16))); }
 };
 
 // Weight of a state with maximum m against the joint maximum M (a state without keys has none).

@@ -1,5 +1,5 @@
 // Paged attention for few rows per K/V head (single tokens, drafts): bounded by the bytes of K and V (64 sequences of 1 to
-// 8192 keys, 32 / 8 heads of 128: 161 us, 6.6 TB/s; 16 of 1024 keys, 32 / 32 heads: 43 us, 6.2 TB/s).
+// 8192 keys, 32 / 8 heads of 128: 160 us, 6.7 TB/s; 16 of 1024 keys, 32 / 32 heads: 43 us, 6.3 TB/s).
 //
 // A unit is (sequence of at most 16 packed rows, K/V head); it has ceil(keys / 64) tiles of 64 keys.  The tiles of all
 // units, end to end, are cut into equal runs, one per CTA, so that ragged batches and one long sequence keep every SM
@@ -10,8 +10,11 @@
 // copies through a ring of its own (no barrier in the loop), S = Q K^T and O += P V run on the tensor pipe
 // (m16n8k16; the packed rows are the 16) and the softmax is one pass with a running maximum.  The ring runs on across
 // units: while one unit's warps are joined and its rows written, the next one's keys are already under way.
-// P is rounded to the cache's type for the second product (half a step, 2^-8 in bf16, of each weight, while l adds
-// the unrounded weights): the errors are independent across keys and stay below the rounding of the output itself.
+// P enters the second product as the sum of two numbers of the cache's type (an error of half a step of half a step, 2^-16 in
+// bf16): rounded once, its error would reach that of the output's own rounding, and the tensor pipe has the room.  Where a
+// call has at most 8 rows a unit, the second parts take the places of rows 8 .. 15 of the same instruction and the two
+// results are added at the unit's end (16 sequences of 1024 keys: 42.7 us against 43.6 by a second product, 43.2 with P rounded
+// once; 64 of 1 to 8192 keys: 159.6, 161.1 and 160.2; capped 160.5, 164.1 and 162.5).
 #include <string>
 
 #include "paged.cuh"
@@ -252,8 +255,9 @@ __device__ __forceinline__ void pr_copy_keys(const PgArgs& a, uint32_t dst, int3
         pr_copy16(d + PR_KEYS * ROW, a.v + src, bytes, once);
     }
 }
-// One tile: the warp's 16 keys, from `first` on, in the stage at ks_s.
-template <typename T, uint32_t HD, bool SCORED>
+// One tile: the warp's 16 keys, from `first` on, in the stage at ks_s.  LIGHT: no unit of the call has more than 8 rows, and
+// the second parts of their weights take the places of rows 8 .. 15.
+template <typename T, uint32_t HD, bool SCORED, bool LIGHT>
 __device__ __forceinline__ void pr_step(const PgArgs& a, uint32_t ks_s, uint32_t first, const uint32_t (&qf)[HD / 16][4], PrState<HD>& u) {
     using S = PrShape<HD>;
     constexpr uint32_t KS = HD / 16, NP = HD / 16;
@@ -276,6 +280,7 @@ __device__ __forceinline__ void pr_step(const PgArgs& a, uint32_t ks_s, uint32_t
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
             const uint32_t r = i >> 1, key = key0 + k * 8 + (i & 1);
+            if (LIGHT && r) continue;
             float x = s[k][i] * a.score_mul;
             if (SCORED) {
                 if (a.cap_mul != 0.0f) x = pg_cap(x, a.cap_mul);
@@ -288,11 +293,15 @@ __device__ __forceinline__ void pr_step(const PgArgs& a, uint32_t ks_s, uint32_t
     float f[2], ms[2];
 #pragma unroll
     for (uint32_t r = 0; r < 2; r++) {
+        if (LIGHT && r) {
+            f[1] = f[0];
+            break;
+        }
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xFFFFFFFFu, mx[r], 1));
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xFFFFFFFFu, mx[r], 2));
         const float mn = fmaxf(u.m[r], mx[r]);
         ms[r] = mn == -INFINITY ? 0.0f : mn;
-        f[r] = pg_exp2(u.m[r] - ms[r]);
+        f[r] = mn == -INFINITY ? 1.0f : pg_exp2(u.m[r] - mn);  // (a row without keys so far has nothing to scale)
         u.m[r] = mn;
         u.l[r] *= f[r];
     }
@@ -305,18 +314,18 @@ __device__ __forceinline__ void pr_step(const PgArgs& a, uint32_t ks_s, uint32_t
             u.o[k][3] *= f[1];
         }
     }
-    uint32_t pf[4];
+    uint32_t pf[4], pl[4];
 #pragma unroll
-    for (uint32_t k = 0; k < 2; k++) {
-        float p[4];
+    for (uint32_t k = 0; k < 2; k++)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            p[i] = pg_exp2(s[k][i] - ms[i >> 1]);
-            u.l[i >> 1] += p[i];
+        for (uint32_t r = 0; r < (LIGHT ? 1 : 2); r++) {
+            const float p0 = pg_exp2(s[k][2 * r] - ms[r]), p1 = pg_exp2(s[k][2 * r + 1] - ms[r]);
+            u.l[r] += p0 + p1;
+            pf[k * 2 + r] = PgType<T>::pack(p0, p1);
+            const float2 h = PgType<T>::widen2(pf[k * 2 + r]);
+            pl[k * 2 + r] = PgType<T>::pack(p0 - h.x, p1 - h.y);
+            if (LIGHT) pf[k * 2 + 1] = pl[k * 2];
         }
-        pf[k * 2] = PgType<T>::pack(p[0], p[1]);
-        pf[k * 2 + 1] = PgType<T>::pack(p[2], p[3]);
-    }
     {
         const uint32_t key = (((lane >> 3) & 1) << 3) | (lane & 7), sub = lane >> 4;
 #pragma unroll
@@ -325,12 +334,23 @@ __device__ __forceinline__ void pr_step(const PgArgs& a, uint32_t ks_s, uint32_t
             pr_ldsm_t(vs_s + key * S::ROW + (((k * 2 + sub) ^ (key & 7)) << 4), vf);
             pr_mma(u.o[2 * k], pf, vf[0], vf[1], T());
             pr_mma(u.o[2 * k + 1], pf, vf[2], vf[3], T());
+            if (!LIGHT) {
+                pr_mma(u.o[2 * k], pl, vf[0], vf[1], T());
+                pr_mma(u.o[2 * k + 1], pl, vf[2], vf[3], T());
+            }
         }
     }
 }
 // The sums of a thread's two rows over the four threads that share them, and the row's (m, l) to ml [2][16].
-template <uint32_t HD> __device__ __forceinline__ void pr_end(PrState<HD>& u, float* ml) {
+template <uint32_t HD, bool LIGHT> __device__ __forceinline__ void pr_end(PrState<HD>& u, float* ml) {
     const uint32_t lane = threadIdx.x & 31, quad = lane >> 2;
+    if (LIGHT) {
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 8; k++) {
+            u.o[k][0] += u.o[k][2];
+            u.o[k][1] += u.o[k][3];
+        }
+    }
 #pragma unroll
     for (uint32_t r = 0; r < 2; r++) {
         u.l[r] += __shfl_xor_sync(0xFFFFFFFFu, u.l[r], 1);
@@ -379,7 +399,7 @@ __device__ __forceinline__ float4 pr_join_warps(const float* j_acc, const float*
     return v;
 }
 
-template <typename T, uint32_t HD, bool SCORED>
+template <typename T, uint32_t HD, bool SCORED, bool LIGHT>
 __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_constant__ PgArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -457,7 +477,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
             pr_wait<S::STAGES - 2>();
             __syncwarp();
             const uint32_t ks_s = ring_s + st * S::STAGE;
-            pr_step<T, HD, SCORED>(a, ks_s, t * PR_TILE + warp * PR_KEYS, qf, u);
+            pr_step<T, HD, SCORED, LIGHT>(a, ks_s, t * PR_TILE + warp * PR_KEYS, qf, u);
             __syncwarp();  // every lane is done with the stage that the next fetch overwrites: the one before this
             fetch(st == 0 ? S::STAGES - 1 : st - 1);
             if (++st == S::STAGES) st = 0;
@@ -468,7 +488,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
         pr_advance(a, kept, seqs, here, n);
         const bool more = here.left != 0;
         if (more) bring_q(here);
-        pr_end<HD>(u, j_ml + warp * 2 * PR_ROWS);
+        pr_end<HD, LIGHT>(u, j_ml + warp * 2 * PR_ROWS);
         float* part = a.parts + ((uint64_t)blockIdx.x * 2 + slot) * S::PART;
         if (!whole && t0 == 0 && tid == 0) {  // a unit that starts here and goes on: what the second kernel joins
             const uint32_t x = first_tile + (whole ? n : pr_tiles(sq)) - 1, cut = run.extra * (run.base + 1);
@@ -510,7 +530,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
 // The same for tables of moderate length, in one launch and without a search: a unit has a cluster of 2^c_log CTAs, each
 // takes an equal range of its tiles, and their states meet in the cluster's shared memory.  Where the call has few rows in
 // all, sequences of up to row_tiles * 16 rows are taken, 16 rows a unit (side by side, so that they share the L2).
-template <typename T, uint32_t HD, bool SCORED>
+template <typename T, uint32_t HD, bool SCORED, bool LIGHT>
 __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_constant__ PgArgs a, uint32_t c_log, uint32_t row_tiles) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -563,13 +583,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_units(const __grid_c
     for (uint32_t t = t0; t < t1; t++) {
         pr_wait<S::STAGES - 2>();
         __syncwarp();
-        pr_step<T, HD, SCORED>(a, ring_s + st * S::STAGE, t * PR_TILE + warp * PR_KEYS, qf, u);
+        pr_step<T, HD, SCORED, LIGHT>(a, ring_s + st * S::STAGE, t * PR_TILE + warp * PR_KEYS, qf, u);
         __syncwarp();
         fetch(st == 0 ? S::STAGES - 1 : st - 1);
         if (++st == S::STAGES) st = 0;
     }
     pr_wait<0>();
-    pr_end<HD>(u, j_ml + warp * 2 * PR_ROWS);
+    pr_end<HD, LIGHT>(u, j_ml + warp * 2 * PR_ROWS);
     // the CTA's state of its rows, in the ring's place (m, l and HD columns a row), then the cluster's
     constexpr uint32_t PER = HD / 4, ROW = HD + 4;
     float* mine = reinterpret_cast<float*>(smem);
@@ -742,35 +762,39 @@ PgRows pg_rows_plan(const PgArgs& a, uint32_t hd, uint32_t sms, uint32_t row_til
     return how;
 }
 
-template <typename T, uint32_t HD, bool SCORED>
+template <typename T, uint32_t HD, bool SCORED, bool LIGHT>
 static qb200_status launch_rows(const PgArgs& a, const PgRows& how, cudaStream_t st) {
     static bool attr_set[64] = {};
     int dev = 0;
     QB_CUDA_TRY(cudaGetDevice(&dev));
     if (!attr_set[dev & 63]) {
-        QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_rows<T, HD, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrShape<HD>::SMEM));
-        QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_units<T, HD, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrShape<HD>::SMEM));
+        QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_rows<T, HD, SCORED, LIGHT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrShape<HD>::SMEM));
+        QB_CUDA_TRY(cudaFuncSetAttribute(k_paged_units<T, HD, SCORED, LIGHT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrShape<HD>::SMEM));
         attr_set[dev & 63] = true;
     }
     const uint32_t grid = how.grid;
     if (how.units) {
-        QB_CUDA_TRY(pg_launch_cluster(k_paged_units<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, 1u << how.c_log, a, how.c_log, how.row_tiles));
+        QB_CUDA_TRY(pg_launch_cluster(k_paged_units<T, HD, SCORED, LIGHT>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, 1u << how.c_log, a, how.c_log, how.row_tiles));
         return QB200_OK;
     }
-    QB_CUDA_TRY(pg_launch(k_paged_rows<T, HD, SCORED>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, a));
+    QB_CUDA_TRY(pg_launch(k_paged_rows<T, HD, SCORED, LIGHT>, dim3(grid), dim3(PR_WARPS * 32), PrShape<HD>::SMEM, st, a));
     const uint64_t rows = a.cu_q || a.shared ? (uint64_t)a.tokens * a.group : a.group;
     QB_CUDA_TRY(pg_launch(k_paged_rows_join<T, HD>, dim3(grid, (uint32_t)((rows < PR_ROWS ? rows : PR_ROWS) + 3) / 4), dim3(512), 0, st, a));
     return QB200_OK;
 }
 
-qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, const PgRows& how, cudaStream_t st) {
+template <typename T, uint32_t HD>
+static qb200_status launch_rows(const PgArgs& a, const PgRows& how, cudaStream_t st) {
     const bool scored = a.cap_mul != 0.0f || a.slopes;
-    if (dtype == QB200_BF16) {
-        if (hd == 128) return scored ? launch_rows<__nv_bfloat16, 128, true>(a, how, st) : launch_rows<__nv_bfloat16, 128, false>(a, how, st);
-        return scored ? launch_rows<__nv_bfloat16, 64, true>(a, how, st) : launch_rows<__nv_bfloat16, 64, false>(a, how, st);
-    }
-    if (hd == 128) return scored ? launch_rows<__half, 128, true>(a, how, st) : launch_rows<__half, 128, false>(a, how, st);
-    return scored ? launch_rows<__half, 64, true>(a, how, st) : launch_rows<__half, 64, false>(a, how, st);
+    // one token a sequence, at most 8 heads a K/V head (or as few rows in all)
+    const bool light = (a.cu_q || a.shared ? (uint64_t)a.tokens * a.group : a.group) <= PR_ROWS / 2;
+    if (light) return scored ? launch_rows<T, HD, true, true>(a, how, st) : launch_rows<T, HD, false, true>(a, how, st);
+    return scored ? launch_rows<T, HD, true, false>(a, how, st) : launch_rows<T, HD, false, false>(a, how, st);
+}
+
+qb200_status pg_rows_launch(const PgArgs& a, int dtype, uint32_t hd, const PgRows& how, cudaStream_t st) {
+    if (dtype == QB200_BF16) return hd == 128 ? launch_rows<__nv_bfloat16, 128>(a, how, st) : launch_rows<__nv_bfloat16, 64>(a, how, st);
+    return hd == 128 ? launch_rows<__half, 128>(a, how, st) : launch_rows<__half, 64>(a, how, st);
 }
 
 }  // namespace qb

@@ -306,3 +306,23 @@ def test_rows_of_nobody_and_of_others_change_no_bit(heads, kv_heads, hd, dtype, 
         got = paged.paged_attention(batch, q, **kw)
         assert torch.equal(got[:first], want[:first]) and torch.equal(got[first + q_lens[1]: rows], want[first + q_lens[1]: rows]), junk
     cache.check()
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF, 128), (FP, 128), (BF, 64), (FP, 64)])
+@pytest.mark.parametrize("width", [0, 2500])
+def test_weights_of_tokens_are_not_rounded_to_the_type(dtype, hd, width):
+    """Few rows: the softmax weights enter the second product as a sum of two numbers of the cache's type.
+
+    The bound is that of paged_reference.attention with u A, the rounding of the weights to the type, replaced by that of the
+    second part: half a step of at most half a step, u^2 A (f16: the second part's smallest step is there already, n 2^-25 max |v|)."""
+    heads, kvh, scale = 8, 2, 0.01  # scores near 0: even weights, and little error from the scores themselves
+    q_lens, kv_lens = [1, 1, 2, 1, 3], [7, 12, 30, 65, 11]
+    m = ref.make(41, q_lens, kv_lens, heads, kvh, hd, 16, dtype, width=width)
+    cache, batch = build(m, kv_lens)
+    out = paged.paged_attention(batch, m["q"].to(DEV), scale=scale)
+    cache.check()
+    want, _, tol, _ = ref.attention(m["q"], m["k"], m["v"], m["table"], kv_lens, m["cu"], heads, scale)
+    mags = dict(m, v=m["v"].abs())
+    A = ref.attention(mags["q"], mags["k"], mags["v"], mags["table"], kv_lens, mags["cu"], heads, scale)[0]  # sum of p |v|
+    u = ref.HALF_STEP[dtype]
+    within(out, want, tol - (u - u * u) * (1 + u) * A)
