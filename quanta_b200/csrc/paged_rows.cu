@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 2) k_paged_rows(const __grid_co
         pr_end<HD, LIGHT>(u, j_ml + warp * 2 * PR_ROWS);
         float* part = a.parts + ((uint64_t)blockIdx.x * 2 + slot) * S::PART;
         if (!whole && t0 == 0 && tid == 0) {  // a unit that starts here and goes on: what the second kernel joins
-            const uint32_t x = first_tile + (whole ? n : pr_tiles(sq)) - 1, cut = run.extra * (run.base + 1);
+            const uint32_t x = first_tile + pr_tiles(sq) - 1, cut = run.extra * (run.base + 1);
             meta[1] = (int32_t)slot;
             meta[2] = (int32_t)sq.q0;
             meta[3] = (int32_t)rows;
