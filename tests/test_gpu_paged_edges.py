@@ -326,3 +326,42 @@ def test_weights_of_tokens_are_not_rounded_to_the_type(dtype, hd, width):
     A = ref.attention(mags["q"], mags["k"], mags["v"], mags["table"], kv_lens, mags["cu"], heads, scale)[0]  # sum of p |v|
     u = ref.HALF_STEP[dtype]
     within(out, want, tol - (u - u * u) * (1 + u) * A)
+
+
+@pytest.mark.parametrize("width", [40, 2500])
+def test_captured_prompts_follow_row_starts_and_lengths(width):
+    """A padded, captured step of append, attention and attention behind a prefix, replayed with other sequences: prompts where tokens
+    were, none at all, more new tokens than keys."""
+    heads, kvh, hd, ps, B, rows, prefix = 8, 2, 128, 16, 3, 420, 50
+    m = ref.make(43, [0] * B, [600] * B, heads, kvh, hd, ps, BF, garbage=0.5, prefix=prefix, width=width)
+    cache, _ = build(m, [600] * B)
+    kv, cu = ints([1, 1, 1]), ints([0, 1, 2, 3])
+    batch = paged.PagedBatch(cache, m["table"].to(DEV), kv, cu)
+    cos, sin = paged.rope_table(700, hd, device=DEV)
+    x = torch.randn(rows, (heads + 2 * kvh) * hd, device=DEV).to(BF)
+    a, b, pre = heads * hd, (heads + kvh) * hd, m["pre"].to(DEV)
+
+    def step():
+        q = paged.paged_rope_append(batch, x[:, :a], x[:, a:b], x[:, b:], cos, sin)
+        return q, paged.paged_attention(batch, q), paged.shared_prefix_attention(batch, q, pre, prefix)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for q_lens, kv_lens in (([1, 1, 1], [5, 600, 90]), ([300, 1, 100], [300, 20, 500]), ([0, 0, 0], [7, 0, 600]), ([1, 419, 0], [0, 30, 9]), ([140, 140, 140], [140, 600, 300])):
+        c = [0]
+        for n in q_lens:
+            c.append(c[-1] + n)
+        kv.copy_(ints(kv_lens))
+        cu.copy_(ints(c))
+        x.copy_(torch.randn_like(x))
+        g.replay()
+        want = step()
+        for w, r in zip(want, got):
+            assert torch.equal(w[: c[-1]], r[: c[-1]])
+    cache.check()
