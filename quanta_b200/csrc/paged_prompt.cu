@@ -15,7 +15,7 @@
 //
 // P is rounded to the cache's type (half a step of each weight, 2^-8 in bf16, while the row's sum adds the unrounded weights): a
 // second product with what the rounding leaves, as the few-rows kernels have it, would make a step's tensor work 1536 cycles
-// of 1024 where the pipe is the bound.  The errors are independent across keys and of the order of the output's own
+// instead of 1024, where the pipe is the bound.  The errors are independent across keys and of the order of the output's own
 // rounding: results differ from the 64-bit definition by 2.0e-3 where rounding alone gives 1.5e-3 (bf16, a prompt of 8192
 // tokens), 2.5e-4 and 2.0e-4 in f16, 2.3e-3 and 1.7e-3 behind a shared prefix of 8192 keys.
 //
